@@ -14,6 +14,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "lcb200_types.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -78,6 +80,69 @@ int lcb_index_fill_f32(float *dst, size_t count, lcbStream stream);
  * ref: the kernel stage between HtoD and DtoH in the reference's stream tests
  * (tests/async_kernels/write_float.cu:1-9 is the reference's stand-in compute kernel). */
 int lcb_axpb_f32(float *y, const float *x, float a, float b, size_t count, lcbStream stream);
+
+/* ---- 8-bit rows: copies that change the number format --------------------------------------------------------
+ *
+ * Format of a row of n values: n e4m3 codes (1 sign, 4 exponent, 3 mantissa bits) and (n + 31) / 32 scale bytes.
+ * 32 consecutive values of a row form a group (the last may be shorter).  With A the largest finite magnitude of a
+ * group its scale is s = 2^(b - 127), where the byte b is the smallest of 0..246 with A <= 448 s (448 is the
+ * largest code; 0 when all values are zero, 246 when 448 * 2^119 < A).  A code is x / s rounded to the
+ * nearest e4m3 value, ties to even, saturating at +-448.  A power of two as scale makes the division exact, so
+ * a code carries exactly one rounding, the result does not depend on how it is computed, and no precision is lost
+ * against a scale that uses the whole range: e4m3 is a floating format.  NaN and both infinities are stored
+ * as the NaN code 0x7f and do not count towards A: a bad value stays visible and spoils no neighbour.
+ * The value of a code is code * s.  Bytes of scale above 246 are never written.  Where an operator returns these
+ * values (lcb_cache_read_q8, lcb_unpack_q8) they are rounded to the wide type once, saturating at its largest
+ * finite value (65504 in f16 may round up to the code for 65536); the NaN code gives NaN.
+ *
+ * `type` is an enum lcbType.  Strides are in elements of the wide type; 0 is allowed for inputs (one row read again and
+ * again); the rows of an output must not overlap (1 is returned).  Wide pointers are aligned to
+ * their element.  Any number of columns, any stride and alignment give the same result; rows whose number of columns,
+ * address and stride are multiples of 16 elements (32 bytes) are fastest, see the kernels.  Inputs and
+ * outputs must not overlap, except that an output of the two silu_mul operators may be exactly an input's rows
+ * (same address and stride).  No workspace is used: calls on several streams may run at once, and a call may be
+ * captured into a CUDA graph (make one call, or lcb_preload, on the device first).  A call with nothing to do returns 0.
+ * ref: none (the reference has no operation that changes a format; driverapi/include/librecuda.h:37-114). */
+
+/* Writes `tokens` rows of keys and values into a paged cache, quantising them: the row of token t, head h,
+ * k + t * k_token_stride + h * k_head_stride, goes to slot slots[t] of the cache (v likewise; v and its strides are ignored
+ * in a cache of one tensor).  `slots` is DEVICE memory, 8-byte aligned.  A negative slot skips its token (a padded batch).  A slot
+ * behind the last page is skipped too and raises bit 2 of the sticky error word (lcb_device_error_word).  Slots that are not
+ * named keep their bytes.  The slots of one call must differ: a slot that is named twice holds an unspecified mix of
+ * the two rows afterwards (no other slot is touched). */
+int lcb_cache_write_q8(const lcbCacheQ8 *cache, const void *k, size_t k_token_stride, size_t k_head_stride, const void *v,
+                       size_t v_token_stride, size_t v_head_stride, int type, const int64_t *slots, size_t tokens,
+                       lcbStream stream);
+
+/* Reads sequences back: for every b < sequences and p < lengths[b], the row of token p % page_tokens of page
+ * page_table[b * table_stride + p / page_tokens] goes, for every head h, to k + (first_rows[b] + p) * k_token_stride + h *
+ * k_head_stride (v likewise).  first_rows places the sequences: running sums of the lengths give a dense ragged batch,
+ * b * max_length a padded one; rows that belong to no sequence keep what they held.  page_table (int32), lengths (int32) and
+ * first_rows (int64) are DEVICE memory; max_length is the host's bound on the lengths (at most table_stride * page_tokens, else
+ * 1 is returned) and sizes the grid; `rows` is the number of rows that k and v have.  A page may stand in several
+ * tables (a shared prefix).  Nothing is read or written out of bounds: a page outside the cache, a row outside
+ * [0, rows), a negative length or one above max_length (read up to max_length) raises bit 2 of the sticky error word,
+ * and the rows concerned keep what they held. */
+int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_token_stride, size_t k_head_stride, void *v, size_t v_token_stride,
+                      size_t v_head_stride, int type, const int32_t *page_table, size_t table_stride, const int32_t *lengths,
+                      const int64_t *first_rows, size_t sequences, size_t max_length, size_t rows, lcbStream stream);
+
+/* Packs a matrix of `rows` rows of `cols` values, src_stride elements apart, into codes [rows][cols] and scales
+ * [rows][(cols + 31) / 32], both dense: an activation kept in 8 bits for the backward pass.  lcb_unpack_q8 is the way back. */
+int lcb_pack_q8(void *codes, void *scales, const void *src, size_t src_stride, int type, size_t rows, size_t cols, lcbStream stream);
+int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void *codes, const void *scales, size_t rows, size_t cols,
+                  lcbStream stream);
+
+/* The gated unit h = gate * up / (1 + exp(-gate)) that leaves its checkpoint in the same pass: `gate` and `up` packed as
+ * lcb_pack_q8 packs them.  h is computed from the wide inputs in 32 bits and rounded once. */
+int lcb_silu_mul_pack_q8(void *h, size_t h_stride, void *gate_codes, void *gate_scales, void *up_codes, void *up_scales, const void *gate,
+                         size_t gate_stride, const void *up, size_t up_stride, int type, size_t rows, size_t cols, lcbStream stream);
+/* Its backward pass from the checkpoint: with g, u the values of the packed gate and up, s = 1 / (1 + exp(-g)) and dh
+ * the gradient of h,   dup = dh * g * s,   dgate = dh * u * s * (1 + g * (1 - s)),   and, unless h is NULL, h = g * s * u again
+ * (for the gradient of the projection behind the unit).  32-bit arithmetic, rounded once. */
+int lcb_silu_mul_grad_q8(void *dgate, size_t dgate_stride, void *dup, size_t dup_stride, void *h, size_t h_stride, const void *dh,
+                         size_t dh_stride, const void *gate_codes, const void *gate_scales, const void *up_codes,
+                         const void *up_scales, int type, size_t rows, size_t cols, lcbStream stream);
 
 /* One rank's half of an all-to-all over peer-mapped buffers, fused into one kernel: for every j in
  * [0, n_ranks) chunk j of `send` (chunk_bytes each) is stored to peer_recv[j] + rank * chunk_bytes.
@@ -202,7 +267,8 @@ int lcb_checksum64_noalloc(const void *src, size_t bytes, uint64_t *out, lcbStre
 size_t lcb_checksum64_noalloc_max_bytes(void);
 
 /* Reads and clears the per-device sticky word that kernels set when a bounded wait gave up: bit 0 an mbarrier
- * wait of the bulk-copy ring, bit 1 a wait for another GPU's flag; 0 = no error.  Synchronises the device. */
+ * wait of the bulk-copy ring, bit 1 a wait for another GPU's flag; bit 2: a cache operator met a slot, page, row or
+ * length out of range and skipped it; 0 = no error.  Synchronises the device. */
 int lcb_device_error_word(unsigned int *out);
 /* The same word as last mirrored into host memory by the kernels, read WITHOUT synchronising or clearing:
  * what a host that has just finished a stream wait consults (libreCuStreamAwait and libreCuEventSynchronize

@@ -22,6 +22,13 @@ lib = C.CDLL(str(LIB_PATH))
 vp, sz, u64, u32, i32 = C.c_void_p, C.c_size_t, C.c_uint64, C.c_uint32, C.c_int
 vpp = C.POINTER(C.c_void_p)
 
+class CacheQ8(C.Structure):
+    """lcbCacheQ8 of include/lcb200_types.h: a paged cache in the 8-bit row format."""
+
+    _fields_ = [("k_codes", vp), ("k_scales", vp), ("v_codes", vp), ("v_scales", vp), ("pages", sz), ("page_tokens", sz),
+                ("heads", sz), ("k_dim", sz), ("v_dim", sz), ("order", i32)]
+
+
 # name -> (restype, argtypes); every symbol the two public headers declare
 LCB_FUNCTIONS = {
     "lcb_copy_d2d": (i32, [vp, vp, sz, vp]),
@@ -33,6 +40,12 @@ LCB_FUNCTIONS = {
     "lcb_memset_ex": (i32, [vp, C.c_uint, i32, sz, i32, i32, vp]),
     "lcb_index_fill_f32": (i32, [vp, sz, vp]),
     "lcb_axpb_f32": (i32, [vp, vp, C.c_float, C.c_float, sz, vp]),
+    "lcb_cache_write_q8": (i32, [C.POINTER(CacheQ8), vp, sz, sz, vp, sz, sz, i32, vp, sz, vp]),
+    "lcb_cache_read_q8": (i32, [C.POINTER(CacheQ8), vp, sz, sz, vp, sz, sz, i32, vp, sz, vp, vp, sz, sz, sz, vp]),
+    "lcb_pack_q8": (i32, [vp, vp, vp, sz, i32, sz, sz, vp]),
+    "lcb_unpack_q8": (i32, [vp, sz, i32, vp, vp, sz, sz, vp]),
+    "lcb_silu_mul_pack_q8": (i32, [vp, sz, vp, vp, vp, vp, vp, sz, vp, sz, i32, sz, sz, vp]),
+    "lcb_silu_mul_grad_q8": (i32, [vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp, vp, i32, sz, sz, vp]),
     "lcb_alltoall_push": (i32, [vpp, vp, sz, i32, i32, vp]),
     "lcb_alltoall_pull": (i32, [vpp, vp, sz, i32, i32, vp]),
     "lcb_multicast_store": (i32, [vp, vp, sz, i32, vp]),

@@ -37,6 +37,11 @@ ATTR_COMPUTE_CAPABILITY_MINOR = 76
 ATTR_MAX_SHARED_MEMORY_PER_BLOCK_OPTIN = 97
 FUNC_ATTR_MAX_DYNAMIC_SHARED_SIZE_BYTES = 8
 
+# element types and cache orders of the 8-bit operators (include/lcb200_types.h)
+F32, F16, BF16 = 0, 1, 2
+CACHE_TOKENS_FIRST, CACHE_HEADS_FIRST = 0, 1
+CacheQ8 = N.CacheQ8
+
 
 class LibreCudaError(RuntimeError):
     def __init__(self, status: int, what: str):

@@ -12,6 +12,14 @@ namespace lcb {
 constexpr unsigned int kErrMbarrierTimeout = 1u;
 // Bit 1: a wait for a flag that another GPU posts gave up.
 constexpr unsigned int kErrFlagTimeout = 2u;
+// Bit 2: a slot, page, row or length given in device memory is out of range; it was skipped.
+constexpr unsigned int kErrIndexRange = 4u;
+// The word and the device variable that holds its host-mapped mirror (NULL before lcb_preload), as kernel arguments.
+struct ErrorSink {
+    unsigned int *word;
+    unsigned int **mirror;
+};
+int error_sink(ErrorSink *out);  // of the current device
 
 // Tunables reachable through lcb_tune() (for sweeps; the defaults are the shipped configuration).
 struct Tuning {
@@ -63,6 +71,7 @@ Tuning &tuning();
 
 int preload_copy_kernels();  // force-load the default copy / fill kernels on the current device
 int preload_fill_kernels();
+int preload_q8_kernels();
 int setup_error_mirror();    // host-mapped mirror of the sticky error word for the current device
 int sm_count();            // SMs of the current device (cached per device)
 int check_launch();        // cudaGetLastError() as int

@@ -1458,6 +1458,25 @@ int setup_error_mirror() {
     g_mirror_host[dev] = h;
     return 0;
 }
+
+// Where kernels of the other sources raise bits of the same word: the device addresses, looked up once per device.
+int error_sink(ErrorSink *out) {
+    static ErrorSink cached[64] = {};
+    int dev = -1;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return (int)err;
+    if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+    if (cached[dev].mirror == nullptr) {
+        void *word = nullptr, *mirror = nullptr;
+        err = cudaGetSymbolAddress(&word, g_error_word);
+        if (err == cudaSuccess) err = cudaGetSymbolAddress(&mirror, g_error_mirror);
+        if (err != cudaSuccess) return (int)err;
+        cached[dev].word = static_cast<unsigned int *>(word);
+        cached[dev].mirror = static_cast<unsigned int **>(mirror);
+    }
+    *out = cached[dev];
+    return 0;
+}
 }  // namespace lcb
 
 extern "C" int lcb_device_error_peek(unsigned int *out) {

@@ -208,6 +208,7 @@ extern "C" int lcb_tune_get(const char *name) {
 extern "C" int lcb_preload(void) {
     int rc = lcb::preload_copy_kernels();
     if (rc == 0) rc = lcb::preload_fill_kernels();
+    if (rc == 0) rc = lcb::preload_q8_kernels();
     if (rc == 0) rc = lcb::setup_error_mirror();
     return rc;
 }
