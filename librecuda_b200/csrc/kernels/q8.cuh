@@ -11,6 +11,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "lcb200_types.h"
 
@@ -37,6 +39,8 @@ struct FastDiv {
 };
 
 // ---- wide elements -------------------------------------------------------------------------------------------
+// A unit is V consecutive values of one row held by one lane: 16 (32-byte accesses), 8 (16-byte accesses) or 1 (any
+// alignment).  32 / V neighbouring lanes hold a group.
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -50,16 +54,101 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// What a read back returns: rounded once, saturating at the type's largest finite value.  The value of a code is at
-// most 448 * 2^119, which only f16 cannot hold; NaN stays NaN.
-template <typename T>
-__device__ __forceinline__ T from_f32_finite(float x) { return from_f32<T>(x); }
-template <>
-__device__ __forceinline__ __half from_f32_finite<__half>(float x) {
+// Two values rounded to a 16-bit type, `lo` in the lower half.  FINITE: saturating at the largest finite value, what a
+// read back returns (the value of a code is at most 448 * 2^119, which only f16 cannot hold; NaN stays NaN).
+template <typename T, bool FINITE>
+__device__ __forceinline__ uint32_t pair_from_f32(float lo, float hi) {
     uint32_t r;
-    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(0.0f), "f"(x));
-    return __ushort_as_half((unsigned short)r);
+    if constexpr (std::is_same_v<T, __half>) {
+        if constexpr (FINITE) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    } else {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    }
+    return r;
 }
+
+template <typename T, int V>
+struct Unit {  // as it lies in memory
+    static constexpr int kWords = V * (int)sizeof(T) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (V == 16) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 8)
+                asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
+                             : "l"(reinterpret_cast<const uint32_t *>(p) + i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {
+                const uint4 v = ld_stream<2>(reinterpret_cast<const uint4 *>(p) + i / 4);
+                w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *p) const {
+        if constexpr (V == 16) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 8)
+                asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                             :: "l"(reinterpret_cast<uint32_t *>(p) + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
+                                "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7]) : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4)
+                st_stream<2>(reinterpret_cast<uint4 *>(p) + i / 4, make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+        }
+    }
+    __device__ __forceinline__ float value(int j) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+        else if constexpr (std::is_same_v<T, __half>) return __half2float(__ushort_as_half((unsigned short)(w[j / 2] >> (16 * (j & 1)))));
+        else return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+    }
+    template <bool FINITE>
+    __device__ __forceinline__ void set(const float (&x)[V]) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(x[i]);
+            else w[i] = pair_from_f32<T, FINITE>(x[2 * i], x[2 * i + 1]);
+        }
+    }
+    // Bits, as f32, of the largest magnitude; those of an infinity or more where an infinity or NaN is among the values.
+    // Magnitudes compare as integers, two 16-bit ones at a time.
+    __device__ __forceinline__ unsigned top_bits() const {
+        if constexpr (sizeof(T) == 4) {
+            unsigned m = 0;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7fffffffu);
+            return m;
+        } else {
+            unsigned m = 0;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+            m = max(m & 0xffffu, m >> 16);
+            if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+            else return m << 16;
+        }
+    }
+};
+template <typename T>
+struct Unit<T, 1> {
+    T x;
+    __device__ __forceinline__ void clear() { x = from_f32<T>(0.0f); }
+    __device__ __forceinline__ void load(const T *p) { x = *p; }
+    __device__ __forceinline__ void store(T *p) const { *p = x; }
+    __device__ __forceinline__ float value(int) const { return to_f32(x); }
+    template <bool FINITE>
+    __device__ __forceinline__ void set(const float (&v)[1]) {
+        if constexpr (FINITE && std::is_same_v<T, __half>) x = __ushort_as_half((unsigned short)pair_from_f32<__half, true>(v[0], 0.0f));
+        else x = from_f32<T>(v[0]);
+    }
+    __device__ __forceinline__ unsigned top_bits() const { return __float_as_uint(to_f32(x)) & 0x7fffffffu; }
+};
 
 // ---- scales and codes ---------------------------------------------------------------------------------------
 __device__ __forceinline__ int scale_byte(unsigned top_bits) {
@@ -75,22 +164,134 @@ __device__ __forceinline__ unsigned finite_magnitude(float x) {
     const unsigned a = __float_as_uint(x) & 0x7fffffffu;
     return a < kInfBits ? a : 0u;
 }
+// infinities are stored as NaN
+__device__ __forceinline__ float nan_if_infinite(float x) {
+    return (__float_as_uint(x) & 0x7fffffffu) == kInfBits ? __uint_as_float(0x7fffffffu) : x;
+}
+
+// largest over the lanes of a group; every lane of the warp calls it
+template <int V>
+__device__ __forceinline__ unsigned group_max(unsigned m) {
+    if constexpr (V == 1) return __reduce_max_sync(0xffffffffu, m);
+    else {
+#pragma unroll
+        for (int o = 1; o < kGroup / V; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        return m;
+    }
+}
 
 __device__ __forceinline__ uint16_t to_codes(float lo, float hi) {  // saturates at +-448, NaN -> 0x7f
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// infinities are stored as NaN
-__device__ __forceinline__ float nan_if_infinite(float x) {
-    return (__float_as_uint(x) & 0x7fffffffu) == kInfBits ? __uint_as_float(0x7fffffffu) : x;
+
+template <int V>
+struct Codes {  // of one unit
+    uint32_t w[(V + 3) / 4];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (V + 3) / 4; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const uint8_t *p) {
+        if constexpr (V == 16) {
+            const uint4 v = ld_stream<2>(reinterpret_cast<const uint4 *>(p));
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else if constexpr (V == 8) {
+            asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+        } else {
+            w[0] = *p;
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t *p) const {
+        if constexpr (V == 16) st_stream<2>(reinterpret_cast<uint4 *>(p), make_uint4(w[0], w[1], w[2], w[3]));
+        else if constexpr (V == 8) asm volatile("st.global.L1::no_allocate.v2.u32 [%0], {%1,%2};" :: "l"(p), "r"(w[0]), "r"(w[1]) : "memory");
+        else *p = (uint8_t)w[0];
+    }
+    // the values, in 32 bits: a code is an f16 value exactly, and its product with a power of two is exact
+    __device__ __forceinline__ void values(float (&x)[V], float scale) const {
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            uint32_t r;
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)(w[j / 4] >> (8 * (j & 2)))));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
+            x[j] = f.x * scale;
+            if constexpr (V > 1) x[j + 1] = f.y * scale;
+        }
+    }
+};
+
+// Packs a unit: its codes, and the scale byte of its group (the same in all lanes of the group).  Every lane of the warp calls
+// it; lanes without values come with a cleared unit.  Infinities and NaN are rare, so the largest magnitude is first
+// taken over everything; only when it is not finite somewhere in the warp the values are looked at one by one.
+template <typename T, int V>
+__device__ __forceinline__ int pack_unit(const Unit<T, V> &in, Codes<V> &out) {
+    float x[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = in.value(j);
+    unsigned top = group_max<V>(in.top_bits());
+    if (__any_sync(0xffffffffu, top >= kInfBits)) {
+        top = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            top = max(top, finite_magnitude(x[j]));
+            x[j] = nan_if_infinite(x[j]);
+        }
+        top = group_max<V>(top);
+    }
+    const int b = scale_byte(top);
+    const float inverse = scale_inverse(b);
+    if constexpr (V == 1) {
+        out.w[0] = to_codes(x[0] * inverse, 0.0f) & 0xffu;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 4)
+            out.w[j / 4] = (uint32_t)to_codes(x[j] * inverse, x[j + 1] * inverse) |
+                           (uint32_t)to_codes(x[j + 2] * inverse, x[j + 3] * inverse) << 16;
+    }
+    return b;
 }
-__device__ __forceinline__ __half2 from_codes(uint16_t c) {  // exact: every code is an f16 value
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
-    return *reinterpret_cast<__half2 *>(&r);
+
+// ---- sigmoid --------------------------------------------------------------------------------------------------
+// s = 1 / (1 + exp(-g)) and q = 1 - s = 1 / (1 + exp(g)), both to a few roundings wherever they are normal numbers: with
+// a = exp(-|g|) <= 1 and r = 1 / (1 + a) one of them is r and the other a * r, so nothing overflows and nothing cancels.
+// exp(-|g|) = 2^-t * (1 - ln2 * rest) with t = |g| log2(e) rounded and the rest of the product kept, since an error of t
+// counts t times.
+struct Sigmoid {
+    float s, q;
+};
+__device__ __forceinline__ Sigmoid sigmoid(float g) {
+    const float m = fminf(fabsf(g), 100.0f);  // exp(-88) is subnormal already; keeps t and rest finite
+    constexpr float kLog2e = 1.4426950216293335f, kLog2eRest = 1.9259629911266175e-8f, kLn2 = 0.69314718246459961f;
+    const float t = m * kLog2e;
+    const float rest = fmaf(m, kLog2eRest, fmaf(m, kLog2e, -t));
+    float a, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(-t));
+    a = fmaf(a * rest, -kLn2, a);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + a));
+    const float ar = a * r;
+    return g >= 0.0f ? Sigmoid{r, ar} : Sigmoid{ar, r};
 }
-__device__ __forceinline__ float from_code(uint8_t c) { return __low2float(from_codes(c)); }
+
+// calls fn with a null pointer of the element type
+template <typename Fn>
+int with_type(int type, Fn fn) {
+    switch (type) {
+        case LCB_F32: return fn(static_cast<float *>(nullptr));
+        case LCB_F16: return fn(static_cast<__half *>(nullptr));
+        default: return fn(static_cast<__nv_bfloat16 *>(nullptr));
+    }
+}
+
+// calls fn with std::integral_constant of the unit
+template <typename Fn>
+int with_unit(int v, Fn fn) {
+    switch (v) {
+        case 16: return fn(std::integral_constant<int, 16>());
+        case 8: return fn(std::integral_constant<int, 8>());
+        default: return fn(std::integral_constant<int, 1>());
+    }
+}
 
 // ---- an index out of range in device memory -----------------------------------------------------------------------
 __device__ __forceinline__ void raise_error(const ErrorSink &e, unsigned bits) {

@@ -1,8 +1,8 @@
 // Paged key/value cache in the 8-bit row format for sm_100a: quantising rows as they are written to their slots, and
 // reading sequences back through a page table.
 //
-// One lane per value, one warp per group, as in q8_rows.cu.  Every index that comes from device memory (slots, pages,
-// lengths, first rows) is checked before it forms an address.
+// Units and groups are those of q8_rows.cu; a row is a token's head here.  Every index that comes from device memory (slots,
+// pages, lengths, first rows) is checked before it forms an address.
 #include "lcb200_kernels.h"
 #include "q8.cuh"
 #include "q8_check.h"
@@ -11,6 +11,7 @@ namespace lcb {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kUnits = 4;  // units in flight per lane
 
 template <typename T>
 struct Side {  // keys or values
@@ -18,8 +19,9 @@ struct Side {  // keys or values
     uint64_t token_stride, head_stride;
     uint8_t *codes, *scales;
     uint64_t dim, groups;
-    FastDiv per_head;   // by the lanes of a row, padded to whole groups
-    uint64_t blocks;    // of the grid (write), or of one sequence (read)
+    FastDiv per_row;                 // by the units of a row, padded to whole groups
+    uint64_t skip_rows, skip_units;  // a CTA's threads as rows and units: from one unit of a lane to its next
+    uint64_t blocks;                 // of the grid (write), or of one sequence (read)
 };
 
 struct Pool {
@@ -32,33 +34,63 @@ struct Pool {
     }
 };
 
-template <typename T>
+template <int V>
+struct Place {  // of a lane's unit among the rows (token, head)
+    uint64_t row, unit;
+    template <typename T>
+    __device__ __forceinline__ Place(const Side<T> &s, uint64_t block) {
+        row = s.per_row.divmod(block * (kThreads * kUnits) + threadIdx.x, unit);
+    }
+    template <typename T>
+    __device__ __forceinline__ void next(const Side<T> &s) {
+        row += s.skip_rows;
+        unit += s.skip_units;
+        if (unit >= s.per_row.d) {
+            unit -= s.per_row.d;
+            ++row;
+        }
+    }
+};
+
+template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) cache_write_kernel(Side<const T> k, Side<const T> v, Pool pool, const int64_t *slots,
                                                                uint64_t tokens, ErrorSink errors) {
     pdl_launch_dependents();
-    pdl_wait();
     const bool first = blockIdx.x < k.blocks;
     const Side<const T> &s = first ? k : v;
-    const uint64_t i = (blockIdx.x - (first ? 0 : k.blocks)) * kThreads + threadIdx.x;
-    uint64_t col, head;
-    const uint64_t token = pool.by_heads.divmod(s.per_head.divmod(i, col), head);
-    if (token >= tokens) return;  // the same for all lanes of a warp
-    const int64_t slot = slots[token];
-    if (slot < 0) return;
-    uint64_t offset;
-    const uint64_t page = pool.page_tokens.divmod((uint64_t)slot, offset);
-    if (page >= pool.pages) {
-        if (col == 0 && head == 0) raise_error(errors, kErrIndexRange);
-        return;
+    Place<V> at(s, blockIdx.x - (first ? 0 : k.blocks));
+    Unit<T, V> x[kUnits];
+    int64_t slot[kUnits];
+    uint64_t head[kUnits], unit[kUnits];
+    pdl_wait();
+    // The rows of skipped tokens are loaded too: waiting for the slot first would put a second memory latency in front of
+    // every row.
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u, at.next(s)) {
+        const uint64_t token = pool.by_heads.divmod(at.row, head[u]);
+        unit[u] = at.unit;
+        slot[u] = -1;
+        x[u].clear();
+        if (token < tokens) {
+            slot[u] = slots[token];
+            if (at.unit * V < s.dim) x[u].load(s.wide + token * s.token_stride + head[u] * s.head_stride + at.unit * V);
+        }
     }
-    const bool in = col < s.dim;
-    const float x = in ? to_f32(s.wide[token * s.token_stride + head * s.head_stride + col]) : 0.0f;
-    const unsigned top = __reduce_max_sync(0xffffffffu, in ? finite_magnitude(x) : 0u);
-    const int b = scale_byte(top);
-    if (!in) return;
-    const uint64_t row = pool.row(page, offset, head);
-    s.codes[row * s.dim + col] = (uint8_t)to_codes(nan_if_infinite(x) * scale_inverse(b), 0.0f);
-    if ((col & (kGroup - 1)) == 0) s.scales[row * s.groups + col / kGroup] = (uint8_t)b;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        Codes<V> c;
+        const int b = pack_unit(x[u], c);
+        if (slot[u] < 0 || unit[u] * V >= s.dim) continue;
+        uint64_t offset;
+        const uint64_t page = pool.page_tokens.divmod((uint64_t)slot[u], offset);
+        if (page >= pool.pages) {
+            if (unit[u] == 0 && head[u] == 0) raise_error(errors, kErrIndexRange);
+            continue;
+        }
+        const uint64_t row = pool.row(page, offset, head[u]);
+        c.store(s.codes + row * s.dim + unit[u] * V);
+        if ((unit[u] & (kGroup / V - 1)) == 0) s.scales[row * s.groups + unit[u] / (kGroup / V)] = (uint8_t)b;
+    }
 }
 
 struct Sequences {
@@ -68,32 +100,55 @@ struct Sequences {
     FastDiv blocks;  // of one sequence, keys and values
 };
 
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(Side<T> k, Side<T> v, Pool pool, Sequences q, ErrorSink errors) {
     pdl_launch_dependents();
-    pdl_wait();
     uint64_t block;
     const uint64_t b = q.blocks.divmod(blockIdx.x, block);
     const bool first = block < k.blocks;
     const Side<T> &s = first ? k : v;
-    const uint64_t i = (block - (first ? 0 : k.blocks)) * kThreads + threadIdx.x;
+    Place<V> at(s, block - (first ? 0 : k.blocks));
+    uint64_t head[kUnits], unit[kUnits], p[kUnits], offset[kUnits];
+    int32_t page[kUnits];
+    pdl_wait();
     const int32_t length = q.lengths[b];
+    const int64_t first_row = q.first_rows[b];
+    // page numbers are loaded beside the length; positions below max_length have an entry in the table
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u, at.next(s)) {
+        p[u] = pool.by_heads.divmod(at.row, head[u]);
+        unit[u] = at.unit;
+        const uint64_t entry = pool.page_tokens.divmod(p[u], offset[u]);
+        page[u] = p[u] < q.max_length ? q.table[b * q.table_stride + entry] : 0;
+    }
     if (block == 0 && threadIdx.x == 0 && (length < 0 || length > (int64_t)q.max_length)) raise_error(errors, kErrIndexRange);
     const uint64_t n = length < 0 ? 0 : min((uint64_t)length, q.max_length);
-    uint64_t col, head, offset;
-    const uint64_t p = pool.by_heads.divmod(s.per_head.divmod(i, col), head);
-    if (p >= n) return;
-    const uint64_t entry = pool.page_tokens.divmod(p, offset);
-    const int32_t page = q.table[b * q.table_stride + entry];
-    const int64_t row = q.first_rows[b] + (int64_t)p;
-    if (page < 0 || (uint64_t)page >= pool.pages || row < 0 || (uint64_t)row >= q.rows) {
-        if (col == 0 && head == 0) raise_error(errors, kErrIndexRange);
-        return;
+    Codes<V> c[kUnits];
+    unsigned scale[kUnits];
+    bool live[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        const int64_t row = first_row + (int64_t)p[u];
+        live[u] = p[u] < n && unit[u] * V < s.dim;
+        if (live[u] && (page[u] < 0 || (uint64_t)page[u] >= pool.pages || row < 0 || (uint64_t)row >= q.rows)) {
+            if (unit[u] == 0 && head[u] == 0) raise_error(errors, kErrIndexRange);
+            live[u] = false;
+        }
+        if (live[u]) {
+            const uint64_t from = pool.row((uint64_t)page[u], offset[u], head[u]);
+            c[u].load(s.codes + from * s.dim + unit[u] * V);
+            scale[u] = s.scales[from * s.groups + unit[u] / (kGroup / V)];
+        }
     }
-    if (col >= s.dim) return;
-    const uint64_t at = pool.row((uint64_t)page, offset, head);
-    const float x = from_code(s.codes[at * s.dim + col]) * scale_value(s.scales[at * s.groups + col / kGroup]);
-    s.wide[(uint64_t)row * s.token_stride + head * s.head_stride + col] = from_f32_finite<T>(x);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        if (!live[u]) continue;
+        float x[V];
+        c[u].values(x, scale_value(scale[u]));
+        Unit<T, V> y;
+        y.template set<true>(x);
+        y.store(s.wide + (uint64_t)(first_row + (int64_t)p[u]) * s.token_stride + head[u] * s.head_stride + unit[u] * V);
+    }
 }
 
 Pool pool_of(const lcbCacheQ8 &c) {
@@ -102,20 +157,40 @@ Pool pool_of(const lcbCacheQ8 &c) {
 
 // `tokens`: rows per head that the side's blocks cover
 template <typename T>
-Side<T> side_of(T *wide, size_t token_stride, size_t head_stride, void *codes, void *scales, size_t dim, const lcbCacheQ8 &c, uint64_t tokens) {
-    if (dim == 0) return {nullptr, 0, 0, nullptr, nullptr, 0, 0, FastDiv::of(1), 0};
-    const uint64_t groups = groups_of(dim), lanes = tokens * c.heads * groups * kGroup;
-    return {wide, token_stride, head_stride, static_cast<uint8_t *>(codes), static_cast<uint8_t *>(scales), dim, groups,
-            FastDiv::of(groups * kGroup), (lanes + kThreads - 1) / kThreads};
+Side<T> side_of(T *wide, size_t token_stride, size_t head_stride, void *codes, void *scales, size_t dim, const lcbCacheQ8 &c, uint64_t tokens,
+                int v) {
+    const uint64_t groups = groups_of(dim), per_row = groups * (kGroup / v), tile = (uint64_t)kThreads * kUnits;
+    return {wide, token_stride, head_stride, static_cast<uint8_t *>(codes), static_cast<uint8_t *>(scales), dim, groups, FastDiv::of(per_row),
+            kThreads / per_row, kThreads % per_row, (tokens * c.heads * per_row + tile - 1) / tile};
 }
 
-template <typename Fn>
-int with_type(int type, Fn fn) {
-    switch (type) {
-        case LCB_F32: return fn(static_cast<float *>(nullptr));
-        case LCB_F16: return fn(static_cast<__half *>(nullptr));
-        default: return fn(static_cast<__nv_bfloat16 *>(nullptr));
+struct Wide {  // the wide tensor of a side, as given
+    const void *p;
+    size_t token_stride, head_stride, dim;
+    void *codes, *scales;
+    // The widest unit whose accesses are aligned in every row (see q8_rows.cu).
+    int unit(const lcbCacheQ8 &c, size_t tokens, size_t e) const {
+        const uint64_t w = reinterpret_cast<uintptr_t>(p) | (tokens > 1 ? token_stride * e : 0) | (c.heads > 1 ? head_stride * e : 0);
+        const uint64_t q = reinterpret_cast<uintptr_t>(codes);
+        if (dim % 16 == 0 && w % 32 == 0 && q % 16 == 0) return 16;
+        if (dim % 8 == 0 && w % 16 == 0 && q % 8 == 0) return 8;
+        return 1;
     }
+};
+
+// Keys and values go to one launch where their units are the same, else to one each.
+// launch(v, k side, v side): either side may have no blocks.
+template <typename T, typename Launch>
+int by_sides(const lcbCacheQ8 &c, const Wide &k, const Wide &v, size_t tokens, size_t rows, Launch launch) {
+    const int ku = k.unit(c, rows, sizeof(T)), vu = c.v_dim != 0 ? v.unit(c, rows, sizeof(T)) : ku;
+    auto side = [&](const Wide &w, int unit, bool on) {
+        if (!on || w.dim == 0) return Side<T>{nullptr, 0, 0, nullptr, nullptr, 0, 0, FastDiv::of(1), 0, 0, 0};
+        return side_of<T>(static_cast<T *>(const_cast<void *>(w.p)), w.token_stride, w.head_stride, w.codes, w.scales, w.dim, c, tokens, unit);
+    };
+    const bool both = ku == vu;
+    const int rc = with_unit(ku, [&](auto u) { return launch(u, side(k, ku, true), side(v, vu, both)); });
+    if (rc != 0 || both) return rc;
+    return with_unit(vu, [&](auto u) { return launch(u, side(k, ku, false), side(v, vu, true)); });
 }
 
 }  // namespace
@@ -136,14 +211,16 @@ extern "C" int lcb_cache_write_q8(const lcbCacheQ8 *cache, const void *k, size_t
     ErrorSink errors;
     const int rc = error_sink(&errors);
     if (rc != 0) return rc;
+    const Wide kw{k, k_token_stride, k_head_stride, cache->k_dim, cache->k_codes, cache->k_scales};
+    const Wide vw{v, v_token_stride, v_head_stride, cache->v_dim, cache->v_codes, cache->v_scales};
     return with_type(type, [&](auto *t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        const auto ks = side_of<const T>(static_cast<const T *>(k), k_token_stride, k_head_stride, cache->k_codes, cache->k_scales, cache->k_dim, *cache, tokens);
-        const auto vs = side_of<const T>(static_cast<const T *>(v), v_token_stride, v_head_stride, cache->v_codes, cache->v_scales, cache->v_dim, *cache, tokens);
-        const uint64_t blocks = ks.blocks + vs.blocks;
-        if (blocks > 0x7fffffffu) return 1;
-        return launch_kernel(cache_write_kernel<T>, (unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(stream), ks, vs, pool_of(*cache),
-                             slots, (uint64_t)tokens, errors);
+        using T = const std::remove_pointer_t<decltype(t)>;
+        return by_sides<T>(*cache, kw, vw, tokens, tokens, [&](auto u, const Side<T> &ks, const Side<T> &vs) {
+            const uint64_t blocks = ks.blocks + vs.blocks;
+            if (blocks > 0x7fffffffu) return 1;
+            return launch_kernel(cache_write_kernel<std::remove_const_t<T>, u()>, (unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(stream),
+                                 ks, vs, pool_of(*cache), slots, (uint64_t)tokens, errors);
+        });
     });
 }
 
@@ -157,14 +234,16 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
     ErrorSink errors;
     const int rc = error_sink(&errors);
     if (rc != 0) return rc;
+    const Wide kw{k, k_token_stride, k_head_stride, cache->k_dim, cache->k_codes, cache->k_scales};
+    const Wide vw{v, v_token_stride, v_head_stride, cache->v_dim, cache->v_codes, cache->v_scales};
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const auto ks = side_of<T>(static_cast<T *>(k), k_token_stride, k_head_stride, cache->k_codes, cache->k_scales, cache->k_dim, *cache, max_length);
-        const auto vs = side_of<T>(static_cast<T *>(v), v_token_stride, v_head_stride, cache->v_codes, cache->v_scales, cache->v_dim, *cache, max_length);
-        const uint64_t each = ks.blocks + vs.blocks;
-        if (each * sequences > 0x7fffffffu) return 1;
-        const Sequences q{page_table, lengths, first_rows, table_stride, max_length, rows, FastDiv::of(each)};
-        return launch_kernel(cache_read_kernel<T>, (unsigned)(each * sequences), kThreads, 0, static_cast<cudaStream_t>(stream), ks, vs,
-                             pool_of(*cache), q, errors);
+        return by_sides<T>(*cache, kw, vw, max_length, rows, [&](auto u, const Side<T> &ks, const Side<T> &vs) {
+            const uint64_t each = ks.blocks + vs.blocks;
+            if (each * sequences > 0x7fffffffu) return 1;
+            const Sequences q{page_table, lengths, first_rows, table_stride, max_length, rows, FastDiv::of(each)};
+            return launch_kernel(cache_read_kernel<T, u()>, (unsigned)(each * sequences), kThreads, 0, static_cast<cudaStream_t>(stream), ks, vs,
+                                 pool_of(*cache), q, errors);
+        });
     });
 }

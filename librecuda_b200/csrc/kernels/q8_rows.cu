@@ -1,8 +1,7 @@
 // 8-bit activation checkpoints for sm_100a: packing and unpacking a matrix, and the gated unit gate * up / (1 + exp(-gate))
 // that leaves its checkpoint in the forward pass and reads it in the backward pass.
 //
-// One lane per value, one warp per group: a warp's 32 lanes hold the 32 consecutive values of a group, so the largest
-// magnitude is one warp-wide maximum over the bits and any number of columns, stride and alignment is the same case.
+// A tile of kUnits units per lane goes to one short CTA; all loads of a tile are issued before its first store.
 #include "lcb200_kernels.h"
 #include "q8.cuh"
 #include "q8_check.h"
@@ -11,6 +10,8 @@ namespace lcb {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kUnits = 4;      // units in flight per lane: pack, unpack
+constexpr int kUnitsSilu = 2;  // the gated unit holds two inputs
 
 template <typename T>
 struct Rows {  // rows of the wide type
@@ -21,107 +22,203 @@ struct Packed {
     uint8_t *codes, *scales;
 };
 
+// The units of a matrix in row order, a row padded to whole groups.
 struct Shape {
-    uint64_t cols, groups;  // per row
-    uint64_t total;         // lanes of all rows, a row padded to whole groups
-    FastDiv per_row;        // by the lanes of a row
-    static Shape of(size_t rows, size_t cols) {
-        const uint64_t groups = groups_of(cols);
-        return {cols, groups, rows * groups * kGroup, FastDiv::of(groups * kGroup)};
+    uint64_t cols, groups;   // per row
+    uint64_t total;          // units
+    FastDiv per_row;         // by the units of a row
+    uint64_t skip_rows, skip_units;  // a CTA's threads as rows and units: from one unit of a lane to its next
+    static Shape of(size_t rows, size_t cols, int v) {
+        const uint64_t groups = groups_of(cols), per_row = groups * (kGroup / v);
+        return {cols, groups, rows * per_row, FastDiv::of(per_row), kThreads / per_row, kThreads % per_row};
     }
 };
 
-struct Lane {
-    uint64_t row, col;
-    bool in;  // a value of the matrix; lanes behind the last column of a row belong to its last group all the same
-    __device__ __forceinline__ Lane(const Shape &s) {
-        const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-        row = s.per_row.divmod(i, col);
-        in = i < s.total && col < s.cols;
+template <int V>
+struct Place {  // of a lane's unit
+    uint64_t row, unit, i;
+    Place() = default;
+    __device__ __forceinline__ Place(const Shape &s, int units) {
+        i = (uint64_t)blockIdx.x * (kThreads * units) + threadIdx.x;
+        row = s.per_row.divmod(i, unit);
     }
+    __device__ __forceinline__ void next(const Shape &s) {
+        i += kThreads;
+        row += s.skip_rows;
+        unit += s.skip_units;
+        if (unit >= s.per_row.d) {
+            unit -= s.per_row.d;
+            ++row;
+        }
+    }
+    // The columns of a unit are all inside the matrix or all behind it.  Lanes behind the last column of a row still
+    // belong to its last group.
+    __device__ __forceinline__ bool in(const Shape &s) const { return i < s.total && unit * V < s.cols; }
+    __device__ __forceinline__ bool leads() const { return (unit & (kGroup / V - 1)) == 0; }
+    __device__ __forceinline__ uint64_t code(const Shape &s) const { return row * s.cols + unit * V; }
+    __device__ __forceinline__ uint64_t scale(const Shape &s) const { return row * s.groups + unit / (kGroup / V); }
+    template <typename T>
+    __device__ __forceinline__ T *wide(const Rows<T> &r) const { return r.p + row * r.stride + unit * V; }
 };
 
-// Called by whole warps: packs the warp's group.
-__device__ __forceinline__ void pack_group(const Packed &out, const Shape &s, const Lane &at, float x) {
-    const unsigned top = __reduce_max_sync(0xffffffffu, at.in ? finite_magnitude(x) : 0u);
-    const int b = scale_byte(top);
-    if (!at.in) return;
-    const uint16_t c = to_codes(nan_if_infinite(x) * scale_inverse(b), 0.0f);
-    out.codes[at.row * s.cols + at.col] = (uint8_t)c;
-    if ((at.col & (kGroup - 1)) == 0) out.scales[at.row * s.groups + at.col / kGroup] = (uint8_t)b;
+template <typename T, int V>
+__device__ __forceinline__ void pack_and_store(const Packed &out, const Shape &s, const Place<V> &at, const Unit<T, V> &x) {
+    Codes<V> c;
+    const int b = pack_unit(x, c);
+    if (!at.in(s)) return;
+    c.store(out.codes + at.code(s));
+    if (at.leads()) out.scales[at.scale(s)] = (uint8_t)b;
 }
 
-__device__ __forceinline__ float unpack_one(const Packed &in, const Shape &s, const Lane &at) {
-    return from_code(in.codes[at.row * s.cols + at.col]) * scale_value(in.scales[at.row * s.groups + at.col / kGroup]);
-}
-
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) pack_kernel(Packed out, Rows<const T> src, Shape s) {
     pdl_launch_dependents();
+    Place<V> at(s, kUnits), place[kUnits];
+    Unit<T, V> x[kUnits];
     pdl_wait();
-    const Lane at(s);
-    const float x = at.in ? to_f32(src.p[at.row * src.stride + at.col]) : 0.0f;
-    pack_group(out, s, at, x);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u, at.next(s)) {
+        place[u] = at;
+        x[u].clear();
+        if (at.in(s)) x[u].load(at.wide(src));
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) pack_and_store(out, s, place[u], x[u]);
 }
 
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) unpack_kernel(Rows<T> dst, Packed in, Shape s) {
     pdl_launch_dependents();
+    Place<V> at(s, kUnits), place[kUnits];
+    Codes<V> c[kUnits];
+    unsigned b[kUnits];
     pdl_wait();
-    const Lane at(s);
-    if (at.in) dst.p[at.row * dst.stride + at.col] = from_f32_finite<T>(unpack_one(in, s, at));
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u, at.next(s)) {
+        place[u] = at;
+        if (at.in(s)) {
+            c[u].load(in.codes + at.code(s));
+            b[u] = in.scales[at.scale(s)];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        if (!place[u].in(s)) continue;
+        float x[V];
+        c[u].values(x, scale_value(b[u]));
+        Unit<T, V> y;
+        y.template set<true>(x);
+        y.store(place[u].wide(dst));
+    }
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
-
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) silu_mul_pack_kernel(Rows<T> h, Packed gate_out, Packed up_out, Rows<const T> gate,
                                                                  Rows<const T> up, Shape s) {
     pdl_launch_dependents();
+    Place<V> at(s, kUnitsSilu), place[kUnitsSilu];
+    Unit<T, V> g[kUnitsSilu], u[kUnitsSilu];
     pdl_wait();
-    const Lane at(s);
-    const float g = at.in ? to_f32(gate.p[at.row * gate.stride + at.col]) : 0.0f;
-    const float u = at.in ? to_f32(up.p[at.row * up.stride + at.col]) : 0.0f;
-    if (at.in) h.p[at.row * h.stride + at.col] = from_f32<T>(g * sigmoid(g) * u);
-    pack_group(gate_out, s, at, g);
-    pack_group(up_out, s, at, u);
+#pragma unroll
+    for (int k = 0; k < kUnitsSilu; ++k, at.next(s)) {
+        place[k] = at;
+        g[k].clear();
+        u[k].clear();
+        if (at.in(s)) {
+            g[k].load(at.wide(gate));
+            u[k].load(at.wide(up));
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kUnitsSilu; ++k) {
+        if (place[k].in(s)) {
+            float y[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) y[j] = g[k].value(j) * sigmoid(g[k].value(j)).s * u[k].value(j);
+            Unit<T, V> out;
+            out.template set<false>(y);
+            out.store(place[k].wide(h));
+        }
+        pack_and_store(gate_out, s, place[k], g[k]);
+        pack_and_store(up_out, s, place[k], u[k]);
+    }
 }
 
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) silu_mul_grad_kernel(Rows<T> dgate, Rows<T> dup, Rows<T> h, Rows<const T> dh, Packed gate,
                                                                  Packed up, Shape s) {
     pdl_launch_dependents();
+    Place<V> at(s, kUnitsSilu), place[kUnitsSilu];
+    Unit<T, V> d[kUnitsSilu];
+    Codes<V> g[kUnitsSilu], u[kUnitsSilu];
+    unsigned gb[kUnitsSilu], ub[kUnitsSilu];
     pdl_wait();
-    const Lane at(s);
-    if (!at.in) return;
-    const float g = unpack_one(gate, s, at), u = unpack_one(up, s, at);
-    const float d = to_f32(dh.p[at.row * dh.stride + at.col]);
-    const float sg = sigmoid(g), silu = g * sg;
-    dup.p[at.row * dup.stride + at.col] = from_f32<T>(d * silu);
-    dgate.p[at.row * dgate.stride + at.col] = from_f32<T>(d * u * (sg + silu * (1.0f - sg)));
-    if (h.p != nullptr) h.p[at.row * h.stride + at.col] = from_f32<T>(silu * u);
+#pragma unroll
+    for (int k = 0; k < kUnitsSilu; ++k, at.next(s)) {
+        place[k] = at;
+        if (at.in(s)) {
+            d[k].load(at.wide(dh));
+            g[k].load(gate.codes + at.code(s));
+            u[k].load(up.codes + at.code(s));
+            gb[k] = gate.scales[at.scale(s)];
+            ub[k] = up.scales[at.scale(s)];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kUnitsSilu; ++k) {
+        if (!place[k].in(s)) continue;
+        float gv[V], uv[V], dg[V], du[V];
+        g[k].values(gv, scale_value(gb[k]));
+        u[k].values(uv, scale_value(ub[k]));
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const Sigmoid sg = sigmoid(gv[j]);
+            const float silu = gv[j] * sg.s, dj = d[k].value(j);
+            du[j] = dj * silu;
+            dg[j] = dj * uv[j] * fmaf(silu, sg.q, sg.s);
+            uv[j] *= silu;
+        }
+        Unit<T, V> out;
+        out.template set<false>(du);
+        out.store(place[k].wide(dup));
+        out.template set<false>(dg);
+        out.store(place[k].wide(dgate));
+        if (h.p != nullptr) {
+            out.template set<false>(uv);
+            out.store(place[k].wide(h));
+        }
+    }
 }
+
+// The widest unit whose accesses are aligned in every row: codes and values of a unit start at multiples of its size.
+// A row's codes lie behind each other, so the columns must be a multiple of the unit; 16 values take 32-byte accesses of the
+// wide type (f32: two) and 16-byte ones of the codes, 8 values half of that.
+struct Fit {
+    uint64_t wide = 0, codes = 0;
+    template <typename T>
+    void add(const Rows<T> &r, size_t rows) {
+        if (r.p != nullptr) wide |= reinterpret_cast<uintptr_t>(r.p) | (rows > 1 ? r.stride * sizeof(T) : 0);
+    }
+    void add(const Packed &p) { codes |= reinterpret_cast<uintptr_t>(p.codes); }
+    int unit(size_t cols) const {
+        if (cols % 16 == 0 && wide % 32 == 0 && codes % 16 == 0) return 16;
+        if (cols % 8 == 0 && wide % 16 == 0 && codes % 8 == 0) return 8;
+        return 1;
+    }
+};
 
 template <typename... KArgs, typename... Args>
-int launch_rows(void (*kernel)(KArgs...), const Shape &s, lcbStream stream, Args... args) {
-    const uint64_t blocks = (s.total + kThreads - 1) / kThreads;
+int launch_rows(void (*kernel)(KArgs...), int units, const Shape &s, lcbStream stream, Args... args) {
+    const uint64_t tile = (uint64_t)kThreads * units, blocks = (s.total + tile - 1) / tile;
     if (blocks > 0x7fffffffu) return 1;
     return launch_kernel(kernel, (unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(stream), args..., s);
-}
-
-// calls fn with a null pointer of the element type
-template <typename Fn>
-int with_type(int type, Fn fn) {
-    switch (type) {
-        case LCB_F32: return fn(static_cast<float *>(nullptr));
-        case LCB_F16: return fn(static_cast<__half *>(nullptr));
-        default: return fn(static_cast<__nv_bfloat16 *>(nullptr));
-    }
 }
 
 Packed packed(const void *codes, const void *scales) {
     return {static_cast<uint8_t *>(const_cast<void *>(codes)), static_cast<uint8_t *>(const_cast<void *>(scales))};
 }
+template <typename T, typename P>
+Rows<T> rows_at(P *p, size_t stride) { return {static_cast<T *>(p), stride}; }
 
 }  // namespace
 }  // namespace lcb
@@ -132,10 +229,16 @@ extern "C" int lcb_pack_q8(void *codes, void *scales, const void *src, size_t sr
                            lcbStream stream) {
     if (!pack_ok(codes, scales, src, src_stride, type, rows, cols, false)) return 1;
     if (rows == 0 || cols == 0) return 0;
-    const Shape s = Shape::of(rows, cols);
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(pack_kernel<T>, s, stream, packed(codes, scales), Rows<const T>{static_cast<const T *>(src), src_stride});
+        const auto in = rows_at<const T>(src, src_stride);
+        const Packed out = packed(codes, scales);
+        Fit fit;
+        fit.add(in, rows);
+        fit.add(out);
+        return with_unit(fit.unit(cols), [&](auto v) {
+            return launch_rows(pack_kernel<T, v()>, kUnits, Shape::of(rows, cols, v()), stream, out, in);
+        });
     });
 }
 
@@ -143,10 +246,16 @@ extern "C" int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void 
                              lcbStream stream) {
     if (!pack_ok(codes, scales, dst, dst_stride, type, rows, cols, true)) return 1;
     if (rows == 0 || cols == 0) return 0;
-    const Shape s = Shape::of(rows, cols);
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(unpack_kernel<T>, s, stream, Rows<T>{static_cast<T *>(dst), dst_stride}, packed(codes, scales));
+        const auto out = rows_at<T>(dst, dst_stride);
+        const Packed in = packed(codes, scales);
+        Fit fit;
+        fit.add(out, rows);
+        fit.add(in);
+        return with_unit(fit.unit(cols), [&](auto v) {
+            return launch_rows(unpack_kernel<T, v()>, kUnits, Shape::of(rows, cols, v()), stream, out, in);
+        });
     });
 }
 
@@ -155,12 +264,20 @@ extern "C" int lcb_silu_mul_pack_q8(void *h, size_t h_stride, void *gate_codes, 
                                     size_t cols, lcbStream stream) {
     if (!silu_pack_ok(h, h_stride, gate_codes, gate_scales, up_codes, up_scales, gate, gate_stride, up, up_stride, type, rows, cols)) return 1;
     if (rows == 0 || cols == 0) return 0;
-    const Shape s = Shape::of(rows, cols);
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(silu_mul_pack_kernel<T>, s, stream, Rows<T>{static_cast<T *>(h), h_stride}, packed(gate_codes, gate_scales),
-                           packed(up_codes, up_scales), Rows<const T>{static_cast<const T *>(gate), gate_stride},
-                           Rows<const T>{static_cast<const T *>(up), up_stride});
+        const auto out = rows_at<T>(h, h_stride);
+        const auto g = rows_at<const T>(gate, gate_stride), u = rows_at<const T>(up, up_stride);
+        const Packed gp = packed(gate_codes, gate_scales), upk = packed(up_codes, up_scales);
+        Fit fit;
+        fit.add(out, rows);
+        fit.add(g, rows);
+        fit.add(u, rows);
+        fit.add(gp);
+        fit.add(upk);
+        return with_unit(fit.unit(cols), [&](auto v) {
+            return launch_rows(silu_mul_pack_kernel<T, v()>, kUnitsSilu, Shape::of(rows, cols, v()), stream, out, gp, upk, g, u);
+        });
     });
 }
 
@@ -171,11 +288,20 @@ extern "C" int lcb_silu_mul_grad_q8(void *dgate, size_t dgate_stride, void *dup,
                       rows, cols))
         return 1;
     if (rows == 0 || cols == 0) return 0;
-    const Shape s = Shape::of(rows, cols);
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return launch_rows(silu_mul_grad_kernel<T>, s, stream, Rows<T>{static_cast<T *>(dgate), dgate_stride},
-                           Rows<T>{static_cast<T *>(dup), dup_stride}, Rows<T>{static_cast<T *>(h), h_stride},
-                           Rows<const T>{static_cast<const T *>(dh), dh_stride}, packed(gate_codes, gate_scales), packed(up_codes, up_scales));
+        const auto dg = rows_at<T>(dgate, dgate_stride), du = rows_at<T>(dup, dup_stride), out = rows_at<T>(h, h_stride);
+        const auto d = rows_at<const T>(dh, dh_stride);
+        const Packed gp = packed(gate_codes, gate_scales), upk = packed(up_codes, up_scales);
+        Fit fit;
+        fit.add(dg, rows);
+        fit.add(du, rows);
+        fit.add(out, rows);
+        fit.add(d, rows);
+        fit.add(gp);
+        fit.add(upk);
+        return with_unit(fit.unit(cols), [&](auto v) {
+            return launch_rows(silu_mul_grad_kernel<T, v()>, kUnitsSilu, Shape::of(rows, cols, v()), stream, dg, du, out, d, gp, upk);
+        });
     });
 }
