@@ -22,8 +22,8 @@ constexpr int kGroup = 32;          // values per scale byte
 constexpr int kMaxScaleByte = 246;  // 448 * 2^(246 - 127) is finite in f32 and bf16, so no value of a code overflows
 constexpr unsigned kInfBits = 0x7f800000u;
 
-// ---- division of a unit index by a launch constant ---------------------------------------------------------
-// magic = floor((2^64 - 1) / d): the high half of n * magic is the quotient or one less, for every 64-bit n.
+// ---- division by a launch constant ----------------------------------------------------------------------------
+// magic = floor((2^bits - 1) / d): the high half of n * magic is the quotient or one less, for every n of `bits` bits.
 struct FastDiv {
     uint64_t magic, d;
     static FastDiv of(uint64_t d) { return {~0ull / d, d}; }
@@ -35,6 +35,69 @@ struct FastDiv {
             ++q;
         }
         return q;
+    }
+};
+struct FastDiv32 {
+    uint32_t magic, d;
+    static FastDiv32 of(uint32_t d) { return {~0u / d, d}; }
+    __device__ __forceinline__ uint32_t divmod(uint32_t n, uint32_t &rest) const {
+        uint32_t q = __umulhi(n, magic);
+        rest = n - q * d;
+        if (rest >= d) {
+            rest -= d;
+            ++q;
+        }
+        return q;
+    }
+};
+
+// ---- which units a lane works on --------------------------------------------------------------------------------
+// The data is `lines` lines (rows of a matrix, tokens of a cache) of `width` units each, a row padded to whole groups.  A
+// CTA takes `passes` lines per lane at the same place of the line, so a lane knows its column once and only steps its pointers
+// from line to line.  Lines of up to kMaxThreads units: several lie side by side in a CTA.  Longer ones: `chunks` CTAs
+// share a line in even parts.  Parts start at multiples of 32 lanes, lines at multiples of a group's lanes, so the lanes of a
+// group are neighbours in one warp.
+constexpr int kMaxThreads = 256;
+struct Tiling {
+    uint64_t width, lines;
+    FastDiv32 by_chunks, by_width;  // by_width: of lines that lie side by side, else 0 / 1
+    uint32_t threads, side_by_side;
+    static Tiling of(uint64_t lines, uint64_t width) {
+        Tiling t{width, lines, FastDiv32::of(1), FastDiv32::of(1), 0, 1};
+        if (width <= kMaxThreads) {
+            t.by_width = FastDiv32::of((uint32_t)width);
+            t.side_by_side = (uint32_t)(kMaxThreads / width);
+            if (t.side_by_side > lines) t.side_by_side = (uint32_t)lines;
+            t.threads = (uint32_t)((t.side_by_side * width + 31) / 32 * 32);
+        } else {
+            const uint64_t chunks = (width + kMaxThreads - 1) / kMaxThreads;
+            t.by_chunks = FastDiv32::of((uint32_t)chunks);
+            t.threads = (uint32_t)(((width + chunks - 1) / chunks + 31) / 32 * 32);
+        }
+        return t;
+    }
+    uint64_t blocks(int passes) const {
+        const uint64_t tile = (uint64_t)side_by_side * passes;
+        return (lines + tile - 1) / tile * by_chunks.d;
+    }
+};
+struct Lane {
+    uint64_t line;  // of the first pass; the next ones are side_by_side further each
+    uint64_t unit;  // of the line
+    bool in;        // has a unit; lanes without one still take part in a warp's votes and shuffles
+    __device__ __forceinline__ Lane(const Tiling &t, uint32_t block, int passes) {
+        uint32_t chunk, place;
+        const uint32_t tile = t.by_chunks.divmod(block, chunk);
+        if (t.by_chunks.d == 1) {
+            const uint32_t local = t.by_width.divmod(threadIdx.x, place);
+            line = (uint64_t)tile * (t.side_by_side * passes) + local;
+            unit = place;
+            in = local < t.side_by_side;
+        } else {
+            line = (uint64_t)tile * passes;
+            unit = (uint64_t)chunk * t.threads + threadIdx.x;
+            in = unit < t.width && threadIdx.x < t.threads;  // a CTA may be wider than this tiling asks for
+        }
     }
 };
 
@@ -117,18 +180,22 @@ struct Unit {  // as it lies in memory
             else w[i] = pair_from_f32<T, FINITE>(x[2 * i], x[2 * i + 1]);
         }
     }
-    // Bits, as f32, of the largest magnitude; those of an infinity or more where an infinity or NaN is among the values.
-    // Magnitudes compare as integers, two 16-bit ones at a time.
+    // Bits, as f32, of the largest magnitude that is not NaN.  16-bit values compare two at a time; the sign that the
+    // instruction leaves is dropped at the end.
     __device__ __forceinline__ unsigned top_bits() const {
         if constexpr (sizeof(T) == 4) {
-            unsigned m = 0;
+            float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7fffffffu);
-            return m;
+            for (int i = 0; i < kWords; ++i) m = fmaxf(m, fabsf(__uint_as_float(w[i])));
+            return __float_as_uint(m);
         } else {
-            unsigned m = 0;
+            uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+            for (int i = 0; i < kWords; ++i) {
+                if constexpr (std::is_same_v<T, __half>) asm("max.xorsign.abs.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i]));
+                else asm("max.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i]));
+            }
+            m &= 0x7fff7fffu;
             m = max(m & 0xffffu, m >> 16);
             if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
             else return m << 16;
@@ -147,7 +214,7 @@ struct Unit<T, 1> {
         if constexpr (FINITE && std::is_same_v<T, __half>) x = __ushort_as_half((unsigned short)pair_from_f32<__half, true>(v[0], 0.0f));
         else x = from_f32<T>(v[0]);
     }
-    __device__ __forceinline__ unsigned top_bits() const { return __float_as_uint(to_f32(x)) & 0x7fffffffu; }
+    __device__ __forceinline__ unsigned top_bits() const { return __float_as_uint(fmaxf(0.0f, fabsf(to_f32(x)))); }
 };
 
 // ---- scales and codes ---------------------------------------------------------------------------------------
@@ -178,6 +245,12 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
         for (int o = 1; o < kGroup / V; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         return m;
     }
+}
+
+// two products in one instruction
+__device__ __forceinline__ void mul2(float a0, float a1, float b, float &r0, float &r1) {
+    asm("{\n.reg .b64 a, b, r;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %4};\nmul.rn.f32x2 r, a, b;\nmov.b64 {%0, %1}, r;\n}"
+        : "=f"(r0), "=f"(r1) : "f"(a0), "f"(a1), "f"(b));
 }
 
 __device__ __forceinline__ uint16_t to_codes(float lo, float hi) {  // saturates at +-448, NaN -> 0x7f
@@ -215,15 +288,15 @@ struct Codes {  // of one unit
             uint32_t r;
             asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)(w[j / 4] >> (8 * (j & 2)))));
             const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
-            x[j] = f.x * scale;
-            if constexpr (V > 1) x[j + 1] = f.y * scale;
+            if constexpr (V > 1) mul2(f.x, f.y, scale, x[j], x[j + 1]);
+            else x[j] = f.x * scale;
         }
     }
 };
 
 // Packs a unit: its codes, and the scale byte of its group (the same in all lanes of the group).  Every lane of the warp calls
-// it; lanes without values come with a cleared unit.  Infinities and NaN are rare, so the largest magnitude is first
-// taken over everything; only when it is not finite somewhere in the warp the values are looked at one by one.
+// it; lanes without values come with a cleared unit.  The maximum ignores NaN, which convert to the NaN code by
+// themselves; infinities are rare, so only when one is found somewhere in the warp the values are looked at one by one.
 template <typename T, int V>
 __device__ __forceinline__ int pack_unit(const Unit<T, V> &in, Codes<V> &out) {
     float x[V];
@@ -245,9 +318,12 @@ __device__ __forceinline__ int pack_unit(const Unit<T, V> &in, Codes<V> &out) {
         out.w[0] = to_codes(x[0] * inverse, 0.0f) & 0xffu;
     } else {
 #pragma unroll
-        for (int j = 0; j < V; j += 4)
-            out.w[j / 4] = (uint32_t)to_codes(x[j] * inverse, x[j + 1] * inverse) |
-                           (uint32_t)to_codes(x[j + 2] * inverse, x[j + 3] * inverse) << 16;
+        for (int j = 0; j < V; j += 4) {
+            float y0, y1, y2, y3;
+            mul2(x[j], x[j + 1], inverse, y0, y1);
+            mul2(x[j + 2], x[j + 3], inverse, y2, y3);
+            out.w[j / 4] = (uint32_t)to_codes(y0, y1) | (uint32_t)to_codes(y2, y3) << 16;
+        }
     }
     return b;
 }

@@ -3,6 +3,8 @@
 //
 // Units and groups are those of q8_rows.cu; a row is a token's head here.  Every index that comes from device memory (slots,
 // pages, lengths, first rows) is checked before it forms an address.
+#include <algorithm>
+
 #include "lcb200_kernels.h"
 #include "q8.cuh"
 #include "q8_check.h"
@@ -10,8 +12,7 @@
 namespace lcb {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kUnits = 4;  // units in flight per lane
+constexpr int kPasses = 4;  // tokens per lane
 
 template <typename T>
 struct Side {  // keys or values
@@ -19,149 +20,149 @@ struct Side {  // keys or values
     uint64_t token_stride, head_stride;
     uint8_t *codes, *scales;
     uint64_t dim, groups;
-    FastDiv per_row;                 // by the units of a row, padded to whole groups
-    uint64_t skip_rows, skip_units;  // a CTA's threads as rows and units: from one unit of a lane to its next
-    uint64_t blocks;                 // of the grid (write), or of one sequence (read)
+    FastDiv32 per_row;  // by the units of a row, padded to whole groups
+    Tiling tiling;      // a line is a token with all its heads
+    uint32_t blocks;    // of the grid (write), or of one sequence (read); 0: no such side in this launch
 };
 
 struct Pool {
-    uint64_t pages, heads;
-    FastDiv page_tokens, by_heads;
+    uint64_t slots, pages, heads;
+    FastDiv page_tokens;      // of a slot
+    FastDiv32 page_tokens32;  // of a position
     int heads_first;
     // row of (page, offset in the page, head)
     __device__ __forceinline__ uint64_t row(uint64_t page, uint64_t offset, uint64_t head) const {
         return heads_first ? (page * heads + head) * page_tokens.d + offset : (page * page_tokens.d + offset) * heads + head;
     }
+    __device__ __forceinline__ uint64_t row_of_slot(uint64_t slot, uint64_t head) const {
+        if (!heads_first) return slot * heads + head;
+        uint64_t offset;
+        const uint64_t page = page_tokens.divmod(slot, offset);
+        return row(page, offset, head);
+    }
 };
 
 template <int V>
-struct Place {  // of a lane's unit among the rows (token, head)
-    uint64_t row, unit;
+struct Place {  // a lane's tokens, and its place in their heads
+    uint64_t token, head, unit, step;
+    bool in_row;
     template <typename T>
-    __device__ __forceinline__ Place(const Side<T> &s, uint64_t block) {
-        row = s.per_row.divmod(block * (kThreads * kUnits) + threadIdx.x, unit);
+    __device__ __forceinline__ Place(const Side<T> &s, uint32_t block) {
+        const Lane lane(s.tiling, block, kPasses);
+        token = lane.line;
+        step = s.tiling.side_by_side;
+        uint32_t u;
+        head = s.per_row.divmod((uint32_t)lane.unit, u);
+        unit = u;
+        in_row = lane.in && unit * V < s.dim;
     }
+    __device__ __forceinline__ bool leads() const { return (unit & (kGroup / V - 1)) == 0; }
     template <typename T>
-    __device__ __forceinline__ void next(const Side<T> &s) {
-        row += s.skip_rows;
-        unit += s.skip_units;
-        if (unit >= s.per_row.d) {
-            unit -= s.per_row.d;
-            ++row;
-        }
+    __device__ __forceinline__ T *wide(const Side<T> &s, uint64_t row) const {
+        return s.wide + row * s.token_stride + head * s.head_stride + unit * V;
     }
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) cache_write_kernel(Side<const T> k, Side<const T> v, Pool pool, const int64_t *slots,
-                                                               uint64_t tokens, ErrorSink errors) {
+__global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> k, Side<const T> v, Pool pool, const int64_t *slots,
+                                                                  uint64_t tokens, ErrorSink errors) {
     pdl_launch_dependents();
     const bool first = blockIdx.x < k.blocks;
     const Side<const T> &s = first ? k : v;
-    Place<V> at(s, blockIdx.x - (first ? 0 : k.blocks));
-    Unit<T, V> x[kUnits];
-    int64_t slot[kUnits];
-    uint64_t head[kUnits], unit[kUnits];
+    const Place<V> at(s, blockIdx.x - (first ? 0 : k.blocks));
+    Unit<T, V> x[kPasses];
+    int64_t slot[kPasses];
     pdl_wait();
     // The rows of skipped tokens are loaded too: waiting for the slot first would put a second memory latency in front of
     // every row.
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u, at.next(s)) {
-        const uint64_t token = pool.by_heads.divmod(at.row, head[u]);
-        unit[u] = at.unit;
+    for (int u = 0; u < kPasses; ++u) {
+        const uint64_t token = at.token + u * at.step;
         slot[u] = -1;
         x[u].clear();
-        if (token < tokens) {
+        if (at.in_row && token < tokens) {
             slot[u] = slots[token];
-            if (at.unit * V < s.dim) x[u].load(s.wide + token * s.token_stride + head[u] * s.head_stride + at.unit * V);
+            x[u].load(at.wide(s, token));
         }
     }
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
+    for (int u = 0; u < kPasses; ++u) {
         Codes<V> c;
         const int b = pack_unit(x[u], c);
-        if (slot[u] < 0 || unit[u] * V >= s.dim) continue;
-        uint64_t offset;
-        const uint64_t page = pool.page_tokens.divmod((uint64_t)slot[u], offset);
-        if (page >= pool.pages) {
-            if (unit[u] == 0 && head[u] == 0) raise_error(errors, kErrIndexRange);
+        if (slot[u] < 0) continue;
+        if ((uint64_t)slot[u] >= pool.slots) {
+            if (at.unit == 0 && at.head == 0) raise_error(errors, kErrIndexRange);
             continue;
         }
-        const uint64_t row = pool.row(page, offset, head[u]);
-        c.store(s.codes + row * s.dim + unit[u] * V);
-        if ((unit[u] & (kGroup / V - 1)) == 0) s.scales[row * s.groups + unit[u] / (kGroup / V)] = (uint8_t)b;
+        const uint64_t row = pool.row_of_slot((uint64_t)slot[u], at.head);
+        c.store(s.codes + row * s.dim + at.unit * V);
+        if (at.leads()) s.scales[row * s.groups + at.unit / (kGroup / V)] = (uint8_t)b;
     }
 }
 
 struct Sequences {
     const int32_t *table, *lengths;
     const int64_t *first_rows;
-    uint64_t table_stride, max_length, rows;
-    FastDiv blocks;  // of one sequence, keys and values
+    uint64_t table_stride, rows;
+    uint32_t max_length;
+    FastDiv32 blocks;  // of one sequence, keys and values
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) cache_read_kernel(Side<T> k, Side<T> v, Pool pool, Sequences q, ErrorSink errors) {
+__global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side<T> v, Pool pool, Sequences q, ErrorSink errors) {
     pdl_launch_dependents();
-    uint64_t block;
-    const uint64_t b = q.blocks.divmod(blockIdx.x, block);
+    uint32_t block;
+    const uint32_t b = q.blocks.divmod(blockIdx.x, block);
     const bool first = block < k.blocks;
     const Side<T> &s = first ? k : v;
-    Place<V> at(s, block - (first ? 0 : k.blocks));
-    uint64_t head[kUnits], unit[kUnits], p[kUnits], offset[kUnits];
-    int32_t page[kUnits];
+    const Place<V> at(s, block - (first ? 0 : k.blocks));
+    const int32_t *table = q.table + b * q.table_stride;
+    uint32_t offset[kPasses];
+    int32_t page[kPasses];
     pdl_wait();
     const int32_t length = q.lengths[b];
     const int64_t first_row = q.first_rows[b];
     // page numbers are loaded beside the length; positions below max_length have an entry in the table
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u, at.next(s)) {
-        p[u] = pool.by_heads.divmod(at.row, head[u]);
-        unit[u] = at.unit;
-        const uint64_t entry = pool.page_tokens.divmod(p[u], offset[u]);
-        page[u] = p[u] < q.max_length ? q.table[b * q.table_stride + entry] : 0;
+    for (int u = 0; u < kPasses; ++u) {
+        const uint64_t p = at.token + u * at.step;
+        const uint32_t entry = pool.page_tokens32.divmod((uint32_t)p, offset[u]);
+        page[u] = p < q.max_length ? table[entry] : 0;
     }
-    if (block == 0 && threadIdx.x == 0 && (length < 0 || length > (int64_t)q.max_length)) raise_error(errors, kErrIndexRange);
-    const uint64_t n = length < 0 ? 0 : min((uint64_t)length, q.max_length);
-    Codes<V> c[kUnits];
-    unsigned scale[kUnits];
-    bool live[kUnits];
+    if (block == 0 && threadIdx.x == 0 && (length < 0 || (uint32_t)length > q.max_length)) raise_error(errors, kErrIndexRange);
+    const uint32_t n = length < 0 ? 0 : min((uint32_t)length, q.max_length);
+    Codes<V> c[kPasses];
+    unsigned scale[kPasses];
+    bool live[kPasses];
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-        const int64_t row = first_row + (int64_t)p[u];
-        live[u] = p[u] < n && unit[u] * V < s.dim;
-        if (live[u] && (page[u] < 0 || (uint64_t)page[u] >= pool.pages || row < 0 || (uint64_t)row >= q.rows)) {
-            if (unit[u] == 0 && head[u] == 0) raise_error(errors, kErrIndexRange);
+    for (int u = 0; u < kPasses; ++u) {
+        const uint64_t p = at.token + u * at.step;
+        const int64_t row = first_row + (int64_t)p;
+        live[u] = at.in_row && p < n;
+        if (live[u] && ((uint32_t)page[u] >= pool.pages || row < 0 || (uint64_t)row >= q.rows)) {
+            if (at.unit == 0 && at.head == 0) raise_error(errors, kErrIndexRange);
             live[u] = false;
         }
         if (live[u]) {
-            const uint64_t from = pool.row((uint64_t)page[u], offset[u], head[u]);
-            c[u].load(s.codes + from * s.dim + unit[u] * V);
-            scale[u] = s.scales[from * s.groups + unit[u] / (kGroup / V)];
+            const uint64_t from = pool.row((uint32_t)page[u], offset[u], at.head);
+            c[u].load(s.codes + from * s.dim + at.unit * V);
+            scale[u] = s.scales[from * s.groups + at.unit / (kGroup / V)];
         }
     }
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
+    for (int u = 0; u < kPasses; ++u) {
         if (!live[u]) continue;
         float x[V];
         c[u].values(x, scale_value(scale[u]));
         Unit<T, V> y;
         y.template set<true>(x);
-        y.store(s.wide + (uint64_t)(first_row + (int64_t)p[u]) * s.token_stride + head[u] * s.head_stride + unit[u] * V);
+        y.store(at.wide(s, (uint64_t)(first_row + (int64_t)(at.token + u * at.step))));
     }
 }
 
 Pool pool_of(const lcbCacheQ8 &c) {
-    return {c.pages, c.heads, FastDiv::of(c.page_tokens), FastDiv::of(c.heads), c.order == LCB_CACHE_HEADS_FIRST};
-}
-
-// `tokens`: rows per head that the side's blocks cover
-template <typename T>
-Side<T> side_of(T *wide, size_t token_stride, size_t head_stride, void *codes, void *scales, size_t dim, const lcbCacheQ8 &c, uint64_t tokens,
-                int v) {
-    const uint64_t groups = groups_of(dim), per_row = groups * (kGroup / v), tile = (uint64_t)kThreads * kUnits;
-    return {wide, token_stride, head_stride, static_cast<uint8_t *>(codes), static_cast<uint8_t *>(scales), dim, groups, FastDiv::of(per_row),
-            kThreads / per_row, kThreads % per_row, (tokens * c.heads * per_row + tile - 1) / tile};
+    return {c.pages * c.page_tokens, c.pages, c.heads, FastDiv::of(c.page_tokens),
+            FastDiv32::of(c.page_tokens > 0xffffffffu ? 0xffffffffu : (uint32_t)c.page_tokens), c.order == LCB_CACHE_HEADS_FIRST};
 }
 
 struct Wide {  // the wide tensor of a side, as given
@@ -184,8 +185,13 @@ template <typename T, typename Launch>
 int by_sides(const lcbCacheQ8 &c, const Wide &k, const Wide &v, size_t tokens, size_t rows, Launch launch) {
     const int ku = k.unit(c, rows, sizeof(T)), vu = c.v_dim != 0 ? v.unit(c, rows, sizeof(T)) : ku;
     auto side = [&](const Wide &w, int unit, bool on) {
-        if (!on || w.dim == 0) return Side<T>{nullptr, 0, 0, nullptr, nullptr, 0, 0, FastDiv::of(1), 0, 0, 0};
-        return side_of<T>(static_cast<T *>(const_cast<void *>(w.p)), w.token_stride, w.head_stride, w.codes, w.scales, w.dim, c, tokens, unit);
+        Side<T> s{};
+        if (!on || w.dim == 0) return s;
+        const uint64_t groups = groups_of(w.dim), per_row = groups * (kGroup / unit);
+        s = {static_cast<T *>(const_cast<void *>(w.p)), w.token_stride, w.head_stride, static_cast<uint8_t *>(w.codes), static_cast<uint8_t *>(w.scales),
+             w.dim, groups, FastDiv32::of((uint32_t)per_row), Tiling::of(tokens, c.heads * per_row), 0};
+        s.blocks = (uint32_t)std::min<uint64_t>(s.tiling.blocks(kPasses), 0x80000000u);  // too many: refused by the launch
+        return s;
     };
     const bool both = ku == vu;
     const int rc = with_unit(ku, [&](auto u) { return launch(u, side(k, ku, true), side(v, vu, both)); });
@@ -216,9 +222,10 @@ extern "C" int lcb_cache_write_q8(const lcbCacheQ8 *cache, const void *k, size_t
     return with_type(type, [&](auto *t) {
         using T = const std::remove_pointer_t<decltype(t)>;
         return by_sides<T>(*cache, kw, vw, tokens, tokens, [&](auto u, const Side<T> &ks, const Side<T> &vs) {
-            const uint64_t blocks = ks.blocks + vs.blocks;
+            const uint64_t blocks = (uint64_t)ks.blocks + vs.blocks;
             if (blocks > 0x7fffffffu) return 1;
-            return launch_kernel(cache_write_kernel<std::remove_const_t<T>, u()>, (unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(stream),
+            const unsigned threads = std::max(ks.tiling.threads, vs.tiling.threads);
+            return launch_kernel(cache_write_kernel<std::remove_const_t<T>, u()>, (unsigned)blocks, threads, 0, static_cast<cudaStream_t>(stream),
                                  ks, vs, pool_of(*cache), slots, (uint64_t)tokens, errors);
         });
     });
@@ -239,10 +246,11 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         return by_sides<T>(*cache, kw, vw, max_length, rows, [&](auto u, const Side<T> &ks, const Side<T> &vs) {
-            const uint64_t each = ks.blocks + vs.blocks;
-            if (each * sequences > 0x7fffffffu) return 1;
-            const Sequences q{page_table, lengths, first_rows, table_stride, max_length, rows, FastDiv::of(each)};
-            return launch_kernel(cache_read_kernel<T, u()>, (unsigned)(each * sequences), kThreads, 0, static_cast<cudaStream_t>(stream), ks, vs,
+            const uint64_t each = (uint64_t)ks.blocks + vs.blocks;
+            if (each > 0x7fffffffu || sequences > 0x7fffffffu / each) return 1;
+            const Sequences q{page_table, lengths, first_rows, table_stride, rows, (uint32_t)max_length, FastDiv32::of((uint32_t)each)};
+            const unsigned threads = std::max(ks.tiling.threads, vs.tiling.threads);
+            return launch_kernel(cache_read_kernel<T, u()>, (unsigned)(each * sequences), threads, 0, static_cast<cudaStream_t>(stream), ks, vs,
                                  pool_of(*cache), q, errors);
         });
     });

@@ -1,7 +1,7 @@
 // 8-bit activation checkpoints for sm_100a: packing and unpacking a matrix, and the gated unit gate * up / (1 + exp(-gate))
 // that leaves its checkpoint in the forward pass and reads it in the backward pass.
 //
-// A tile of kUnits units per lane goes to one short CTA; all loads of a tile are issued before its first store.
+// All loads of a CTA are issued before its first store.
 #include "lcb200_kernels.h"
 #include "q8.cuh"
 #include "q8_check.h"
@@ -9,9 +9,8 @@
 namespace lcb {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kUnits = 4;      // units in flight per lane: pack, unpack
-constexpr int kUnitsSilu = 2;  // the gated unit holds two inputs
+constexpr int kPasses = 4;      // units in flight per lane: pack, unpack
+constexpr int kPassesSilu = 2;  // the gated unit holds two inputs
 
 template <typename T>
 struct Rows {  // rows of the wide type
@@ -22,151 +21,139 @@ struct Packed {
     uint8_t *codes, *scales;
 };
 
-// The units of a matrix in row order, a row padded to whole groups.
 struct Shape {
-    uint64_t cols, groups;   // per row
-    uint64_t total;          // units
-    FastDiv per_row;         // by the units of a row
-    uint64_t skip_rows, skip_units;  // a CTA's threads as rows and units: from one unit of a lane to its next
+    uint64_t rows, cols, groups;
+    Tiling tiling;
     static Shape of(size_t rows, size_t cols, int v) {
-        const uint64_t groups = groups_of(cols), per_row = groups * (kGroup / v);
-        return {cols, groups, rows * per_row, FastDiv::of(per_row), kThreads / per_row, kThreads % per_row};
+        const uint64_t groups = groups_of(cols);
+        return {rows, cols, groups, Tiling::of(rows, groups * (kGroup / v))};
     }
 };
 
+// A lane's column and its rows.  The columns of a unit are all inside the matrix or all behind it; lanes behind the last
+// column of a row still belong to its last group.
 template <int V>
-struct Place {  // of a lane's unit
-    uint64_t row, unit, i;
-    Place() = default;
-    __device__ __forceinline__ Place(const Shape &s, int units) {
-        i = (uint64_t)blockIdx.x * (kThreads * units) + threadIdx.x;
-        row = s.per_row.divmod(i, unit);
+struct Place {
+    uint64_t row, unit, rows, step;
+    bool in_row;
+    __device__ __forceinline__ Place(const Shape &s, int passes) {
+        const Lane lane(s.tiling, blockIdx.x, passes);
+        row = lane.line;
+        unit = lane.unit;
+        rows = s.rows;
+        step = s.tiling.side_by_side;
+        in_row = lane.in && unit * V < s.cols;
     }
-    __device__ __forceinline__ void next(const Shape &s) {
-        i += kThreads;
-        row += s.skip_rows;
-        unit += s.skip_units;
-        if (unit >= s.per_row.d) {
-            unit -= s.per_row.d;
-            ++row;
-        }
-    }
-    // The columns of a unit are all inside the matrix or all behind it.  Lanes behind the last column of a row still
-    // belong to its last group.
-    __device__ __forceinline__ bool in(const Shape &s) const { return i < s.total && unit * V < s.cols; }
+    __device__ __forceinline__ bool in(int pass) const { return in_row && row + pass * step < rows; }
     __device__ __forceinline__ bool leads() const { return (unit & (kGroup / V - 1)) == 0; }
-    __device__ __forceinline__ uint64_t code(const Shape &s) const { return row * s.cols + unit * V; }
-    __device__ __forceinline__ uint64_t scale(const Shape &s) const { return row * s.groups + unit / (kGroup / V); }
+    __device__ __forceinline__ uint64_t code(const Shape &s, int pass) const { return (row + pass * step) * s.cols + unit * V; }
+    __device__ __forceinline__ uint64_t scale(const Shape &s, int pass) const { return (row + pass * step) * s.groups + unit / (kGroup / V); }
     template <typename T>
-    __device__ __forceinline__ T *wide(const Rows<T> &r) const { return r.p + row * r.stride + unit * V; }
+    __device__ __forceinline__ T *wide(const Rows<T> &r, int pass) const { return r.p + (row + pass * step) * r.stride + unit * V; }
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void pack_and_store(const Packed &out, const Shape &s, const Place<V> &at, const Unit<T, V> &x) {
+__device__ __forceinline__ void pack_and_store(const Packed &out, const Shape &s, const Place<V> &at, int pass, const Unit<T, V> &x) {
     Codes<V> c;
     const int b = pack_unit(x, c);
-    if (!at.in(s)) return;
-    c.store(out.codes + at.code(s));
-    if (at.leads()) out.scales[at.scale(s)] = (uint8_t)b;
+    if (!at.in(pass)) return;
+    c.store(out.codes + at.code(s, pass));
+    if (at.leads()) out.scales[at.scale(s, pass)] = (uint8_t)b;
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) pack_kernel(Packed out, Rows<const T> src, Shape s) {
+__global__ void __launch_bounds__(kMaxThreads) pack_kernel(Packed out, Rows<const T> src, Shape s) {
     pdl_launch_dependents();
-    Place<V> at(s, kUnits), place[kUnits];
-    Unit<T, V> x[kUnits];
+    const Place<V> at(s, kPasses);
+    Unit<T, V> x[kPasses];
     pdl_wait();
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u, at.next(s)) {
-        place[u] = at;
+    for (int u = 0; u < kPasses; ++u) {
         x[u].clear();
-        if (at.in(s)) x[u].load(at.wide(src));
+        if (at.in(u)) x[u].load(at.wide(src, u));
     }
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) pack_and_store(out, s, place[u], x[u]);
+    for (int u = 0; u < kPasses; ++u) pack_and_store(out, s, at, u, x[u]);
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) unpack_kernel(Rows<T> dst, Packed in, Shape s) {
+__global__ void __launch_bounds__(kMaxThreads) unpack_kernel(Rows<T> dst, Packed in, Shape s) {
     pdl_launch_dependents();
-    Place<V> at(s, kUnits), place[kUnits];
-    Codes<V> c[kUnits];
-    unsigned b[kUnits];
+    const Place<V> at(s, kPasses);
+    Codes<V> c[kPasses];
+    unsigned b[kPasses];
     pdl_wait();
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u, at.next(s)) {
-        place[u] = at;
-        if (at.in(s)) {
-            c[u].load(in.codes + at.code(s));
-            b[u] = in.scales[at.scale(s)];
+    for (int u = 0; u < kPasses; ++u) {
+        if (at.in(u)) {
+            c[u].load(in.codes + at.code(s, u));
+            b[u] = in.scales[at.scale(s, u)];
         }
     }
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-        if (!place[u].in(s)) continue;
+    for (int u = 0; u < kPasses; ++u) {
+        if (!at.in(u)) continue;
         float x[V];
         c[u].values(x, scale_value(b[u]));
         Unit<T, V> y;
         y.template set<true>(x);
-        y.store(place[u].wide(dst));
+        y.store(at.wide(dst, u));
     }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) silu_mul_pack_kernel(Rows<T> h, Packed gate_out, Packed up_out, Rows<const T> gate,
-                                                                 Rows<const T> up, Shape s) {
+__global__ void __launch_bounds__(kMaxThreads) silu_mul_pack_kernel(Rows<T> h, Packed gate_out, Packed up_out, Rows<const T> gate,
+                                                                    Rows<const T> up, Shape s) {
     pdl_launch_dependents();
-    Place<V> at(s, kUnitsSilu), place[kUnitsSilu];
-    Unit<T, V> g[kUnitsSilu], u[kUnitsSilu];
+    const Place<V> at(s, kPassesSilu);
+    Unit<T, V> g[kPassesSilu], u[kPassesSilu];
     pdl_wait();
 #pragma unroll
-    for (int k = 0; k < kUnitsSilu; ++k, at.next(s)) {
-        place[k] = at;
+    for (int k = 0; k < kPassesSilu; ++k) {
         g[k].clear();
         u[k].clear();
-        if (at.in(s)) {
-            g[k].load(at.wide(gate));
-            u[k].load(at.wide(up));
+        if (at.in(k)) {
+            g[k].load(at.wide(gate, k));
+            u[k].load(at.wide(up, k));
         }
     }
 #pragma unroll
-    for (int k = 0; k < kUnitsSilu; ++k) {
-        if (place[k].in(s)) {
+    for (int k = 0; k < kPassesSilu; ++k) {
+        if (at.in(k)) {
             float y[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) y[j] = g[k].value(j) * sigmoid(g[k].value(j)).s * u[k].value(j);
             Unit<T, V> out;
             out.template set<false>(y);
-            out.store(place[k].wide(h));
+            out.store(at.wide(h, k));
         }
-        pack_and_store(gate_out, s, place[k], g[k]);
-        pack_and_store(up_out, s, place[k], u[k]);
+        pack_and_store(gate_out, s, at, k, g[k]);
+        pack_and_store(up_out, s, at, k, u[k]);
     }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) silu_mul_grad_kernel(Rows<T> dgate, Rows<T> dup, Rows<T> h, Rows<const T> dh, Packed gate,
-                                                                 Packed up, Shape s) {
+__global__ void __launch_bounds__(kMaxThreads) silu_mul_grad_kernel(Rows<T> dgate, Rows<T> dup, Rows<T> h, Rows<const T> dh, Packed gate,
+                                                                    Packed up, Shape s) {
     pdl_launch_dependents();
-    Place<V> at(s, kUnitsSilu), place[kUnitsSilu];
-    Unit<T, V> d[kUnitsSilu];
-    Codes<V> g[kUnitsSilu], u[kUnitsSilu];
-    unsigned gb[kUnitsSilu], ub[kUnitsSilu];
+    const Place<V> at(s, kPassesSilu);
+    Unit<T, V> d[kPassesSilu];
+    Codes<V> g[kPassesSilu], u[kPassesSilu];
+    unsigned gb[kPassesSilu], ub[kPassesSilu];
     pdl_wait();
 #pragma unroll
-    for (int k = 0; k < kUnitsSilu; ++k, at.next(s)) {
-        place[k] = at;
-        if (at.in(s)) {
-            d[k].load(at.wide(dh));
-            g[k].load(gate.codes + at.code(s));
-            u[k].load(up.codes + at.code(s));
-            gb[k] = gate.scales[at.scale(s)];
-            ub[k] = up.scales[at.scale(s)];
+    for (int k = 0; k < kPassesSilu; ++k) {
+        if (at.in(k)) {
+            d[k].load(at.wide(dh, k));
+            g[k].load(gate.codes + at.code(s, k));
+            u[k].load(up.codes + at.code(s, k));
+            gb[k] = gate.scales[at.scale(s, k)];
+            ub[k] = up.scales[at.scale(s, k)];
         }
     }
 #pragma unroll
-    for (int k = 0; k < kUnitsSilu; ++k) {
-        if (!place[k].in(s)) continue;
+    for (int k = 0; k < kPassesSilu; ++k) {
+        if (!at.in(k)) continue;
         float gv[V], uv[V], dg[V], du[V];
         g[k].values(gv, scale_value(gb[k]));
         u[k].values(uv, scale_value(ub[k]));
@@ -180,12 +167,12 @@ __global__ void __launch_bounds__(kThreads) silu_mul_grad_kernel(Rows<T> dgate, 
         }
         Unit<T, V> out;
         out.template set<false>(du);
-        out.store(place[k].wide(dup));
+        out.store(at.wide(dup, k));
         out.template set<false>(dg);
-        out.store(place[k].wide(dgate));
+        out.store(at.wide(dgate, k));
         if (h.p != nullptr) {
             out.template set<false>(uv);
-            out.store(place[k].wide(h));
+            out.store(at.wide(h, k));
         }
     }
 }
@@ -208,10 +195,10 @@ struct Fit {
 };
 
 template <typename... KArgs, typename... Args>
-int launch_rows(void (*kernel)(KArgs...), int units, const Shape &s, lcbStream stream, Args... args) {
-    const uint64_t tile = (uint64_t)kThreads * units, blocks = (s.total + tile - 1) / tile;
+int launch_rows(void (*kernel)(KArgs...), int passes, const Shape &s, lcbStream stream, Args... args) {
+    const uint64_t blocks = s.tiling.blocks(passes);
     if (blocks > 0x7fffffffu) return 1;
-    return launch_kernel(kernel, (unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(stream), args..., s);
+    return launch_kernel(kernel, (unsigned)blocks, s.tiling.threads, 0, static_cast<cudaStream_t>(stream), args..., s);
 }
 
 Packed packed(const void *codes, const void *scales) {
@@ -237,7 +224,7 @@ extern "C" int lcb_pack_q8(void *codes, void *scales, const void *src, size_t sr
         fit.add(in, rows);
         fit.add(out);
         return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(pack_kernel<T, v()>, kUnits, Shape::of(rows, cols, v()), stream, out, in);
+            return launch_rows(pack_kernel<T, v()>, kPasses, Shape::of(rows, cols, v()), stream, out, in);
         });
     });
 }
@@ -254,7 +241,7 @@ extern "C" int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void 
         fit.add(out, rows);
         fit.add(in);
         return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(unpack_kernel<T, v()>, kUnits, Shape::of(rows, cols, v()), stream, out, in);
+            return launch_rows(unpack_kernel<T, v()>, kPasses, Shape::of(rows, cols, v()), stream, out, in);
         });
     });
 }
@@ -276,7 +263,7 @@ extern "C" int lcb_silu_mul_pack_q8(void *h, size_t h_stride, void *gate_codes, 
         fit.add(gp);
         fit.add(upk);
         return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(silu_mul_pack_kernel<T, v()>, kUnitsSilu, Shape::of(rows, cols, v()), stream, out, gp, upk, g, u);
+            return launch_rows(silu_mul_pack_kernel<T, v()>, kPassesSilu, Shape::of(rows, cols, v()), stream, out, gp, upk, g, u);
         });
     });
 }
@@ -301,7 +288,7 @@ extern "C" int lcb_silu_mul_grad_q8(void *dgate, size_t dgate_stride, void *dup,
         fit.add(gp);
         fit.add(upk);
         return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(silu_mul_grad_kernel<T, v()>, kUnitsSilu, Shape::of(rows, cols, v()), stream, dg, du, out, d, gp, upk);
+            return launch_rows(silu_mul_grad_kernel<T, v()>, kPassesSilu, Shape::of(rows, cols, v()), stream, dg, du, out, d, gp, upk);
         });
     });
 }
