@@ -101,6 +101,34 @@ struct Lane {
     }
 };
 
+// ---- pairs: two 32-bit operations in one instruction ----------------------------------------------------------------
+struct Pair {
+    uint64_t v;
+    Pair() = default;
+    __device__ __forceinline__ Pair(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+    __device__ __forceinline__ explicit Pair(float x) : Pair(x, x) {}
+    __device__ __forceinline__ float2 get() const {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
 // ---- wide elements -------------------------------------------------------------------------------------------
 // A unit is V consecutive values of one row held by one lane: 16 (32-byte accesses), 8 (16-byte accesses) or 1 (any
 // alignment).  32 / V neighbouring lanes hold a group.
@@ -172,13 +200,12 @@ struct Unit {  // as it lies in memory
         else if constexpr (std::is_same_v<T, __half>) return __half2float(__ushort_as_half((unsigned short)(w[j / 2] >> (16 * (j & 1)))));
         else return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
     }
+    __device__ __forceinline__ Pair pair(int j) const { return Pair(value(j), value(j + 1)); }  // j even
     template <bool FINITE>
-    __device__ __forceinline__ void set(const float (&x)[V]) {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(x[i]);
-            else w[i] = pair_from_f32<T, FINITE>(x[2 * i], x[2 * i + 1]);
-        }
+    __device__ __forceinline__ void set_pair(int j, Pair x) {
+        const float2 f = x.get();
+        if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(f.x), w[j + 1] = __float_as_uint(f.y);
+        else w[j / 2] = pair_from_f32<T, FINITE>(f.x, f.y);
     }
     // Bits, as f32, of the largest magnitude that is not NaN.  16-bit values compare two at a time; the sign that the
     // instruction leaves is dropped at the end.
@@ -209,10 +236,11 @@ struct Unit<T, 1> {
     __device__ __forceinline__ void load(const T *p) { x = *p; }
     __device__ __forceinline__ void store(T *p) const { *p = x; }
     __device__ __forceinline__ float value(int) const { return to_f32(x); }
+    __device__ __forceinline__ Pair pair(int) const { return Pair(to_f32(x), 0.0f); }
     template <bool FINITE>
-    __device__ __forceinline__ void set(const float (&v)[1]) {
-        if constexpr (FINITE && std::is_same_v<T, __half>) x = __ushort_as_half((unsigned short)pair_from_f32<__half, true>(v[0], 0.0f));
-        else x = from_f32<T>(v[0]);
+    __device__ __forceinline__ void set_pair(int, Pair v) {
+        if constexpr (FINITE && std::is_same_v<T, __half>) x = __ushort_as_half((unsigned short)pair_from_f32<__half, true>(v.get().x, 0.0f));
+        else x = from_f32<T>(v.get().x);
     }
     __device__ __forceinline__ unsigned top_bits() const { return __float_as_uint(fmaxf(0.0f, fabsf(to_f32(x)))); }
 };
@@ -247,12 +275,6 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
     }
 }
 
-// two products in one instruction
-__device__ __forceinline__ void mul2(float a0, float a1, float b, float &r0, float &r1) {
-    asm("{\n.reg .b64 a, b, r;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %4};\nmul.rn.f32x2 r, a, b;\nmov.b64 {%0, %1}, r;\n}"
-        : "=f"(r0), "=f"(r1) : "f"(a0), "f"(a1), "f"(b));
-}
-
 __device__ __forceinline__ uint16_t to_codes(float lo, float hi) {  // saturates at +-448, NaN -> 0x7f
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
@@ -281,16 +303,12 @@ struct Codes {  // of one unit
         else if constexpr (V == 8) asm volatile("st.global.L1::no_allocate.v2.u32 [%0], {%1,%2};" :: "l"(p), "r"(w[0]), "r"(w[1]) : "memory");
         else *p = (uint8_t)w[0];
     }
-    // the values, in 32 bits: a code is an f16 value exactly, and its product with a power of two is exact
-    __device__ __forceinline__ void values(float (&x)[V], float scale) const {
-#pragma unroll
-        for (int j = 0; j < V; j += 2) {
-            uint32_t r;
-            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)(w[j / 4] >> (8 * (j & 2)))));
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
-            if constexpr (V > 1) mul2(f.x, f.y, scale, x[j], x[j + 1]);
-            else x[j] = f.x * scale;
-        }
+    // values j and j + 1 (j even), in 32 bits: a code is an f16 value exactly, and its product with a power of two is exact
+    __device__ __forceinline__ Pair pair(int j, float scale) const {
+        uint32_t r;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)(w[j / 4] >> (8 * (j & 2)))));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
+        return Pair(f.x, f.y) * Pair(scale);
     }
 };
 
@@ -319,34 +337,38 @@ __device__ __forceinline__ int pack_unit(const Unit<T, V> &in, Codes<V> &out) {
     } else {
 #pragma unroll
         for (int j = 0; j < V; j += 4) {
-            float y0, y1, y2, y3;
-            mul2(x[j], x[j + 1], inverse, y0, y1);
-            mul2(x[j + 2], x[j + 3], inverse, y2, y3);
-            out.w[j / 4] = (uint32_t)to_codes(y0, y1) | (uint32_t)to_codes(y2, y3) << 16;
+            const float2 lo = (Pair(x[j], x[j + 1]) * Pair(inverse)).get(), hi = (Pair(x[j + 2], x[j + 3]) * Pair(inverse)).get();
+            out.w[j / 4] = (uint32_t)to_codes(lo.x, lo.y) | (uint32_t)to_codes(hi.x, hi.y) << 16;
         }
     }
     return b;
 }
 
 // ---- sigmoid --------------------------------------------------------------------------------------------------
-// s = 1 / (1 + exp(-g)) and q = 1 - s = 1 / (1 + exp(g)), both to a few roundings wherever they are normal numbers: with
-// a = exp(-|g|) <= 1 and r = 1 / (1 + a) one of them is r and the other a * r, so nothing overflows and nothing cancels.
-// exp(-|g|) = 2^-t * (1 - ln2 * rest) with t = |g| log2(e) rounded and the rest of the product kept, since an error of t
-// counts t times.
+// s = 1 / (1 + e) and q = 1 - s = e * s with e = exp(-g): no term cancels, so both are good to a few roundings wherever they
+// are normal numbers.  g is held to [-88, 100]: below, s is subnormal and becomes 0; above, e does.  e is finite for all of
+// them, and an infinite or NaN g still shows in g * s.
+// e = 2^t * (1 - ln2 * rest) with t = -g log2(e) rounded and rest what the rounding left of g log2(e), since an error of t
+// counts |t| times.
 struct Sigmoid {
-    float s, q;
+    Pair s, q;
 };
-__device__ __forceinline__ Sigmoid sigmoid(float g) {
-    const float m = fminf(fabsf(g), 100.0f);  // exp(-88) is subnormal already; keeps t and rest finite
+__device__ __forceinline__ Sigmoid sigmoid(Pair g) {
     constexpr float kLog2e = 1.4426950216293335f, kLog2eRest = 1.9259629911266175e-8f, kLn2 = 0.69314718246459961f;
-    const float t = m * kLog2e;
-    const float rest = fmaf(m, kLog2eRest, fmaf(m, kLog2e, -t));
-    float a, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(-t));
-    a = fmaf(a * rest, -kLn2, a);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + a));
-    const float ar = a * r;
-    return g >= 0.0f ? Sigmoid{r, ar} : Sigmoid{ar, r};
+    const float2 f = g.get();
+    const Pair m(fminf(fmaxf(f.x, -88.0f), 100.0f), fminf(fmaxf(f.y, -88.0f), 100.0f));
+    const Pair t = m * Pair(-kLog2e);
+    const Pair rest = fma2(m, Pair(kLog2eRest), fma2(m, Pair(kLog2e), t));
+    float2 e = t.get();
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+    Pair p(e.x, e.y);
+    p = fma2(p * rest, Pair(-kLn2), p);
+    float2 d = (p + Pair(1.0f)).get();
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.y));
+    const Pair s(d.x, d.y);
+    return {s, p * s};
 }
 
 // calls fn with a null pointer of the element type

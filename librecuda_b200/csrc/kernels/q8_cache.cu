@@ -17,49 +17,43 @@ constexpr int kPasses = 4;  // tokens per lane
 template <typename T>
 struct Side {  // keys or values
     T *wide;
-    uint64_t token_stride, head_stride;
+    uint64_t token_stride, head_stride;  // in elements of the wide type
     uint8_t *codes, *scales;
-    uint64_t dim, groups;
-    FastDiv32 per_row;  // by the units of a row, padded to whole groups
-    Tiling tiling;      // a line is a token with all its heads
-    uint32_t blocks;    // of the grid (write), or of one sequence (read); 0: no such side in this launch
+    uint32_t dim, groups;
+    uint32_t token_rows, head_rows;  // rows of the pool from token to token and from head to head of a page
+    FastDiv32 per_row;               // by the units of a row, padded to whole groups
+    Tiling tiling;                   // a line is a token with all its heads
+    uint32_t blocks;                 // of the grid (write), or of one sequence (read); 0: no such side in this launch
 };
 
 struct Pool {
-    uint64_t slots, pages, heads;
-    FastDiv page_tokens;      // of a slot
-    FastDiv32 page_tokens32;  // of a position
-    int heads_first;
-    // row of (page, offset in the page, head)
-    __device__ __forceinline__ uint64_t row(uint64_t page, uint64_t offset, uint64_t head) const {
-        return heads_first ? (page * heads + head) * page_tokens.d + offset : (page * page_tokens.d + offset) * heads + head;
-    }
-    __device__ __forceinline__ uint64_t row_of_slot(uint64_t slot, uint64_t head) const {
-        if (!heads_first) return slot * heads + head;
-        uint64_t offset;
-        const uint64_t page = page_tokens.divmod(slot, offset);
-        return row(page, offset, head);
-    }
+    uint64_t slots, pages, page_rows;  // rows of a page: its tokens times the heads
+    FastDiv page_tokens;               // of a slot
+    FastDiv32 page_tokens32;           // of a position
+    bool heads_first;
 };
 
+// A lane's tokens and its place in their heads.
 template <int V>
-struct Place {  // a lane's tokens, and its place in their heads
-    uint64_t token, head, unit, step;
-    bool in_row;
+struct Place {
+    uint64_t token, wide;    // wide: offset of the lane's values from the token's
+    uint64_t code, scale;    // the same in the pool
+    uint32_t step;
+    bool in_row, leads, first;
     template <typename T>
     __device__ __forceinline__ Place(const Side<T> &s, uint32_t block) {
         const Lane lane(s.tiling, block, kPasses);
         token = lane.line;
         step = s.tiling.side_by_side;
-        uint32_t u;
-        head = s.per_row.divmod((uint32_t)lane.unit, u);
-        unit = u;
+        uint32_t unit;
+        const uint32_t head = s.per_row.divmod((uint32_t)lane.unit, unit);
+        const uint64_t row = (uint64_t)head * s.head_rows;
+        wide = head * s.head_stride + unit * V;
+        code = row * s.dim + unit * V;
+        scale = row * s.groups + unit / (kGroup / V);
         in_row = lane.in && unit * V < s.dim;
-    }
-    __device__ __forceinline__ bool leads() const { return (unit & (kGroup / V - 1)) == 0; }
-    template <typename T>
-    __device__ __forceinline__ T *wide(const Side<T> &s, uint64_t row) const {
-        return s.wide + row * s.token_stride + head * s.head_stride + unit * V;
+        leads = (unit & (kGroup / V - 1)) == 0;
+        first = lane.unit == 0;
     }
 };
 
@@ -67,9 +61,10 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> k, Side<const T> v, Pool pool, const int64_t *slots,
                                                                   uint64_t tokens, ErrorSink errors) {
     pdl_launch_dependents();
-    const bool first = blockIdx.x < k.blocks;
-    const Side<const T> &s = first ? k : v;
-    const Place<V> at(s, blockIdx.x - (first ? 0 : k.blocks));
+    const bool keys = blockIdx.x < k.blocks;
+    const Side<const T> s = keys ? k : v;
+    const Place<V> at(s, blockIdx.x - (keys ? 0 : k.blocks));
+    const T *from = s.wide + at.token * s.token_stride + at.wide;
     Unit<T, V> x[kPasses];
     int64_t slot[kPasses];
     pdl_wait();
@@ -82,7 +77,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
         x[u].clear();
         if (at.in_row && token < tokens) {
             slot[u] = slots[token];
-            x[u].load(at.wide(s, token));
+            x[u].load(from + u * (at.step * s.token_stride));
         }
     }
 #pragma unroll
@@ -91,12 +86,17 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
         const int b = pack_unit(x[u], c);
         if (slot[u] < 0) continue;
         if ((uint64_t)slot[u] >= pool.slots) {
-            if (at.unit == 0 && at.head == 0) raise_error(errors, kErrIndexRange);
+            if (at.first) raise_error(errors, kErrIndexRange);
             continue;
         }
-        const uint64_t row = pool.row_of_slot((uint64_t)slot[u], at.head);
-        c.store(s.codes + row * s.dim + at.unit * V);
-        if (at.leads()) s.scales[row * s.groups + at.unit / (kGroup / V)] = (uint8_t)b;
+        uint64_t row = (uint64_t)slot[u] * s.token_rows;
+        if (pool.heads_first) {
+            uint64_t offset;
+            row = pool.page_tokens.divmod((uint64_t)slot[u], offset) * pool.page_rows;
+            row += offset;
+        }
+        c.store(s.codes + row * s.dim + at.code);
+        if (at.leads) s.scales[row * s.groups + at.scale] = (uint8_t)b;
     }
 }
 
@@ -113,9 +113,9 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
     pdl_launch_dependents();
     uint32_t block;
     const uint32_t b = q.blocks.divmod(blockIdx.x, block);
-    const bool first = block < k.blocks;
-    const Side<T> &s = first ? k : v;
-    const Place<V> at(s, block - (first ? 0 : k.blocks));
+    const bool keys = block < k.blocks;
+    const Side<T> s = keys ? k : v;
+    const Place<V> at(s, block - (keys ? 0 : k.blocks));
     const int32_t *table = q.table + b * q.table_stride;
     uint32_t offset[kPasses];
     int32_t page[kPasses];
@@ -125,44 +125,44 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
     // page numbers are loaded beside the length; positions below max_length have an entry in the table
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
-        const uint64_t p = at.token + u * at.step;
-        const uint32_t entry = pool.page_tokens32.divmod((uint32_t)p, offset[u]);
+        const uint32_t p = (uint32_t)at.token + u * at.step;
+        const uint32_t entry = pool.page_tokens32.divmod(p, offset[u]);
         page[u] = p < q.max_length ? table[entry] : 0;
     }
     if (block == 0 && threadIdx.x == 0 && (length < 0 || (uint32_t)length > q.max_length)) raise_error(errors, kErrIndexRange);
     const uint32_t n = length < 0 ? 0 : min((uint32_t)length, q.max_length);
+    const int64_t row = first_row + (int64_t)at.token;
+    T *to = s.wide + (uint64_t)row * s.token_stride + at.wide;  // not formed into an access before its row is checked
     Codes<V> c[kPasses];
     unsigned scale[kPasses];
     bool live[kPasses];
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
-        const uint64_t p = at.token + u * at.step;
-        const int64_t row = first_row + (int64_t)p;
+        const uint32_t p = (uint32_t)at.token + u * at.step;
         live[u] = at.in_row && p < n;
-        if (live[u] && ((uint32_t)page[u] >= pool.pages || row < 0 || (uint64_t)row >= q.rows)) {
-            if (at.unit == 0 && at.head == 0) raise_error(errors, kErrIndexRange);
+        if (live[u] && ((uint32_t)page[u] >= pool.pages || (uint64_t)(row + (int64_t)(u * at.step)) >= q.rows)) {
+            if (at.first) raise_error(errors, kErrIndexRange);
             live[u] = false;
         }
         if (live[u]) {
-            const uint64_t from = pool.row((uint32_t)page[u], offset[u], at.head);
-            c[u].load(s.codes + from * s.dim + at.unit * V);
-            scale[u] = s.scales[from * s.groups + at.unit / (kGroup / V)];
+            const uint64_t from = (uint32_t)page[u] * pool.page_rows + (uint64_t)offset[u] * s.token_rows;
+            c[u].load(s.codes + from * s.dim + at.code);
+            scale[u] = s.scales[from * s.groups + at.scale];
         }
     }
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
         if (!live[u]) continue;
-        float x[V];
-        c[u].values(x, scale_value(scale[u]));
         Unit<T, V> y;
-        y.template set<true>(x);
-        y.store(at.wide(s, (uint64_t)(first_row + (int64_t)(at.token + u * at.step))));
+#pragma unroll
+        for (int j = 0; j < V; j += 2) y.template set_pair<true>(j, c[u].pair(j, scale_value(scale[u])));
+        y.store(to + u * (at.step * s.token_stride));
     }
 }
 
 Pool pool_of(const lcbCacheQ8 &c) {
-    return {c.pages * c.page_tokens, c.pages, c.heads, FastDiv::of(c.page_tokens),
-            FastDiv32::of(c.page_tokens > 0xffffffffu ? 0xffffffffu : (uint32_t)c.page_tokens), c.order == LCB_CACHE_HEADS_FIRST};
+    return {c.pages * c.page_tokens, c.pages, c.page_tokens * c.heads, FastDiv::of(c.page_tokens),
+            FastDiv32::of((uint32_t)c.page_tokens), c.order == LCB_CACHE_HEADS_FIRST};
 }
 
 struct Wide {  // the wide tensor of a side, as given
@@ -188,8 +188,10 @@ int by_sides(const lcbCacheQ8 &c, const Wide &k, const Wide &v, size_t tokens, s
         Side<T> s{};
         if (!on || w.dim == 0) return s;
         const uint64_t groups = groups_of(w.dim), per_row = groups * (kGroup / unit);
+        const bool heads_first = c.order == LCB_CACHE_HEADS_FIRST;
         s = {static_cast<T *>(const_cast<void *>(w.p)), w.token_stride, w.head_stride, static_cast<uint8_t *>(w.codes), static_cast<uint8_t *>(w.scales),
-             w.dim, groups, FastDiv32::of((uint32_t)per_row), Tiling::of(tokens, c.heads * per_row), 0};
+             (uint32_t)w.dim, (uint32_t)groups, heads_first ? 1u : (uint32_t)c.heads, heads_first ? (uint32_t)c.page_tokens : 1u,
+             FastDiv32::of((uint32_t)per_row), Tiling::of(tokens, c.heads * per_row), 0};
         s.blocks = (uint32_t)std::min<uint64_t>(s.tiling.blocks(kPasses), 0x80000000u);  // too many: refused by the launch
         return s;
     };

@@ -79,7 +79,8 @@ inline bool cache_ok(const lcbCacheQ8 *c) {
     if ((c->v_codes != nullptr) != two || (c->v_scales != nullptr) != two) return false;
     size_t slots;
     if (__builtin_mul_overflow(c->pages, c->page_tokens, &slots) || (slots >> 62)) return false;
-    // a token's rows together stay below 2^31 values, padded: positions within a token are 32-bit numbers
+    // a token's rows together stay below 2^31 values, padded, and a page below 2^31 tokens: both are 32-bit numbers
+    if (c->page_tokens > (size_t)INT32_MAX) return false;
     for (size_t dim : {c->k_dim, c->v_dim})
         if (dim > (size_t)INT32_MAX - 31 || c->heads > ((size_t)1 << 31) / 32 / (groups_of(dim) + 1)) return false;
     return product_ok(slots, c->heads, groups_of(c->k_dim), 32) &&

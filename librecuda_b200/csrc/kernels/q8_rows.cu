@@ -11,6 +11,7 @@ namespace {
 
 constexpr int kPasses = 4;      // units in flight per lane: pack, unpack
 constexpr int kPassesSilu = 2;  // the gated unit holds two inputs
+constexpr int kPassesGrad = 1;  // and its gradient three, with three outputs
 
 template <typename T>
 struct Rows {  // rows of the wide type
@@ -34,22 +35,27 @@ struct Shape {
 // column of a row still belong to its last group.
 template <int V>
 struct Place {
-    uint64_t row, unit, rows, step;
+    uint64_t row, unit, left;  // left: rows from `row` on
+    uint32_t step;
     bool in_row;
     __device__ __forceinline__ Place(const Shape &s, int passes) {
         const Lane lane(s.tiling, blockIdx.x, passes);
         row = lane.line;
         unit = lane.unit;
-        rows = s.rows;
         step = s.tiling.side_by_side;
-        in_row = lane.in && unit * V < s.cols;
+        in_row = lane.in && unit * V < s.cols && row < s.rows;
+        left = s.rows - row;
     }
-    __device__ __forceinline__ bool in(int pass) const { return in_row && row + pass * step < rows; }
+    __device__ __forceinline__ bool in(int pass) const { return in_row && pass * step < left; }
     __device__ __forceinline__ bool leads() const { return (unit & (kGroup / V - 1)) == 0; }
-    __device__ __forceinline__ uint64_t code(const Shape &s, int pass) const { return (row + pass * step) * s.cols + unit * V; }
-    __device__ __forceinline__ uint64_t scale(const Shape &s, int pass) const { return (row + pass * step) * s.groups + unit / (kGroup / V); }
+    __device__ __forceinline__ uint8_t *code(const Packed &p, const Shape &s, int pass) const {
+        return p.codes + (row * s.cols + unit * V) + pass * (step * s.cols);
+    }
+    __device__ __forceinline__ uint8_t *scale(const Packed &p, const Shape &s, int pass) const {
+        return p.scales + (row * s.groups + unit / (kGroup / V)) + pass * (step * s.groups);
+    }
     template <typename T>
-    __device__ __forceinline__ T *wide(const Rows<T> &r, int pass) const { return r.p + (row + pass * step) * r.stride + unit * V; }
+    __device__ __forceinline__ T *wide(const Rows<T> &r, int pass) const { return r.p + (row * r.stride + unit * V) + pass * (step * r.stride); }
 };
 
 template <typename T, int V>
@@ -57,8 +63,8 @@ __device__ __forceinline__ void pack_and_store(const Packed &out, const Shape &s
     Codes<V> c;
     const int b = pack_unit(x, c);
     if (!at.in(pass)) return;
-    c.store(out.codes + at.code(s, pass));
-    if (at.leads()) out.scales[at.scale(s, pass)] = (uint8_t)b;
+    c.store(at.code(out, s, pass));
+    if (at.leads()) *at.scale(out, s, pass) = (uint8_t)b;
 }
 
 template <typename T, int V>
@@ -86,17 +92,16 @@ __global__ void __launch_bounds__(kMaxThreads) unpack_kernel(Rows<T> dst, Packed
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
         if (at.in(u)) {
-            c[u].load(in.codes + at.code(s, u));
-            b[u] = in.scales[at.scale(s, u)];
+            c[u].load(at.code(in, s, u));
+            b[u] = *at.scale(in, s, u);
         }
     }
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
         if (!at.in(u)) continue;
-        float x[V];
-        c[u].values(x, scale_value(b[u]));
         Unit<T, V> y;
-        y.template set<true>(x);
+#pragma unroll
+        for (int j = 0; j < V; j += 2) y.template set_pair<true>(j, c[u].pair(j, scale_value(b[u])));
         y.store(at.wide(dst, u));
     }
 }
@@ -120,11 +125,12 @@ __global__ void __launch_bounds__(kMaxThreads) silu_mul_pack_kernel(Rows<T> h, P
 #pragma unroll
     for (int k = 0; k < kPassesSilu; ++k) {
         if (at.in(k)) {
-            float y[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) y[j] = g[k].value(j) * sigmoid(g[k].value(j)).s * u[k].value(j);
             Unit<T, V> out;
-            out.template set<false>(y);
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+                const Pair x = g[k].pair(j);
+                out.template set_pair<false>(j, x * sigmoid(x).s * u[k].pair(j));
+            }
             out.store(at.wide(h, k));
         }
         pack_and_store(gate_out, s, at, k, g[k]);
@@ -132,48 +138,42 @@ __global__ void __launch_bounds__(kMaxThreads) silu_mul_pack_kernel(Rows<T> h, P
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool AGAIN>
 __global__ void __launch_bounds__(kMaxThreads) silu_mul_grad_kernel(Rows<T> dgate, Rows<T> dup, Rows<T> h, Rows<const T> dh, Packed gate,
                                                                     Packed up, Shape s) {
     pdl_launch_dependents();
-    const Place<V> at(s, kPassesSilu);
-    Unit<T, V> d[kPassesSilu];
-    Codes<V> g[kPassesSilu], u[kPassesSilu];
-    unsigned gb[kPassesSilu], ub[kPassesSilu];
+    const Place<V> at(s, kPassesGrad);
+    Unit<T, V> d[kPassesGrad];
+    Codes<V> g[kPassesGrad], u[kPassesGrad];
+    unsigned gb[kPassesGrad], ub[kPassesGrad];
     pdl_wait();
 #pragma unroll
-    for (int k = 0; k < kPassesSilu; ++k) {
+    for (int k = 0; k < kPassesGrad; ++k) {
         if (at.in(k)) {
             d[k].load(at.wide(dh, k));
-            g[k].load(gate.codes + at.code(s, k));
-            u[k].load(up.codes + at.code(s, k));
-            gb[k] = gate.scales[at.scale(s, k)];
-            ub[k] = up.scales[at.scale(s, k)];
+            g[k].load(at.code(gate, s, k));
+            u[k].load(at.code(up, s, k));
+            gb[k] = *at.scale(gate, s, k);
+            ub[k] = *at.scale(up, s, k);
         }
     }
 #pragma unroll
-    for (int k = 0; k < kPassesSilu; ++k) {
+    for (int k = 0; k < kPassesGrad; ++k) {
         if (!at.in(k)) continue;
-        float gv[V], uv[V], dg[V], du[V];
-        g[k].values(gv, scale_value(gb[k]));
-        u[k].values(uv, scale_value(ub[k]));
+        const float gs = scale_value(gb[k]), us = scale_value(ub[k]);
+        Unit<T, V> dg, du, y;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const Sigmoid sg = sigmoid(gv[j]);
-            const float silu = gv[j] * sg.s, dj = d[k].value(j);
-            du[j] = dj * silu;
-            dg[j] = dj * uv[j] * fmaf(silu, sg.q, sg.s);
-            uv[j] *= silu;
+        for (int j = 0; j < V; j += 2) {
+            const Pair x = g[k].pair(j, gs), z = u[k].pair(j, us), dj = d[k].pair(j);
+            const Sigmoid sg = sigmoid(x);
+            const Pair silu = x * sg.s;
+            du.template set_pair<false>(j, dj * silu);
+            dg.template set_pair<false>(j, dj * z * fma2(silu, sg.q, sg.s));
+            if constexpr (AGAIN) y.template set_pair<false>(j, silu * z);
         }
-        Unit<T, V> out;
-        out.template set<false>(du);
-        out.store(at.wide(dup, k));
-        out.template set<false>(dg);
-        out.store(at.wide(dgate, k));
-        if (h.p != nullptr) {
-            out.template set<false>(uv);
-            out.store(at.wide(h, k));
-        }
+        du.store(at.wide(dup, k));
+        dg.store(at.wide(dgate, k));
+        if constexpr (AGAIN) y.store(at.wide(h, k));
     }
 }
 
@@ -288,7 +288,8 @@ extern "C" int lcb_silu_mul_grad_q8(void *dgate, size_t dgate_stride, void *dup,
         fit.add(gp);
         fit.add(upk);
         return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(silu_mul_grad_kernel<T, v()>, kPassesSilu, Shape::of(rows, cols, v()), stream, dg, du, out, d, gp, upk);
+            return launch_rows(h != nullptr ? silu_mul_grad_kernel<T, v(), true> : silu_mul_grad_kernel<T, v(), false>, kPassesGrad,
+                               Shape::of(rows, cols, v()), stream, dg, du, out, d, gp, upk);
         });
     });
 }
