@@ -51,19 +51,41 @@ struct FastDiv32 {
     }
 };
 
+// ---- units --------------------------------------------------------------------------------------------------------
+// A unit is what one lane holds of a row, in one of three forms V.  V = 16 or 8: that many consecutive values, moved by 32- or
+// 16-byte accesses of the wide type; 32 / V neighbouring lanes hold a group.  V = 1, for rows at any alignment: eight
+// values 32 columns apart, so that a warp holds eight groups, each access of the warp covers the values of one group side
+// by side, and the maximum of a group is one warp-wide instruction.
+constexpr int kStridedValues = 8;
+template <int V>
+struct Form {
+    static constexpr int kValues = V == 1 ? kStridedValues : V;
+    static constexpr int kScales = V == 1 ? kStridedValues : 1;  // groups that a unit has a part of
+    static constexpr int kLanes = kGroup / V;                    // lanes that share them
+    __host__ __device__ static uint64_t per_row(uint64_t groups) {
+        return V == 1 ? (groups + kStridedValues - 1) / kStridedValues * kGroup : groups * kLanes;
+    }
+    __device__ static __forceinline__ uint64_t column(uint64_t unit) {
+        return V == 1 ? unit / kGroup * (kGroup * kStridedValues) + unit % kGroup : unit * V;
+    }
+    __device__ static __forceinline__ uint64_t scale(uint64_t unit) { return V == 1 ? unit / kGroup * kStridedValues : unit / kLanes; }
+    __device__ static __forceinline__ bool leads(uint64_t unit) { return unit % kLanes == 0; }  // writes the scales
+};
+
 // ---- which units a lane works on --------------------------------------------------------------------------------
 // The data is `lines` lines (rows of a matrix, tokens of a cache) of `width` units each, a row padded to whole groups.  A
-// CTA takes `passes` lines per lane at the same place of the line, so a lane knows its column once and only steps its pointers
-// from line to line.  Lines of up to kMaxThreads units: several lie side by side in a CTA.  Longer ones: `chunks` CTAs
-// share a line in even parts.  Parts start at multiples of 32 lanes, lines at multiples of a group's lanes, so the lanes of a
-// group are neighbours in one warp.
-constexpr int kMaxThreads = 256;
+// CTA takes `passes` units per lane, at the same place of as many lines, so a lane knows its column once and only steps its
+// pointers from line to line.  Lines of up to kMaxThreads units: several lie side by side in a CTA.  Longer ones: `chunks`
+// CTAs share a line in even parts.  Parts start at multiples of 32 lanes, lines at multiples of a group's lanes, so
+// the lanes of a group are neighbours in one warp.  Little work is spread over more CTAs with fewer passes.
+constexpr int kMaxThreads = 128;
 struct Tiling {
     uint64_t width, lines;
     FastDiv32 by_chunks, by_width;  // by_width: of lines that lie side by side, else 0 / 1
-    uint32_t threads, side_by_side;
-    static Tiling of(uint64_t lines, uint64_t width) {
-        Tiling t{width, lines, FastDiv32::of(1), FastDiv32::of(1), 0, 1};
+    uint32_t threads, side_by_side, passes;
+    // `times`: how often the launch repeats the tiling
+    static Tiling of(uint64_t lines, uint64_t width, uint32_t max_passes, uint64_t times = 1) {
+        Tiling t{width, lines, FastDiv32::of(1), FastDiv32::of(1), 0, 1, 1};
         if (width <= kMaxThreads) {
             t.by_width = FastDiv32::of((uint32_t)width);
             t.side_by_side = (uint32_t)(kMaxThreads / width);
@@ -74,9 +96,11 @@ struct Tiling {
             t.by_chunks = FastDiv32::of((uint32_t)chunks);
             t.threads = (uint32_t)(((width + chunks - 1) / chunks + 31) / 32 * 32);
         }
+        const uint64_t resident = (uint64_t)sm_count() * (2048 / kMaxThreads);
+        while (t.passes < max_passes && lines > (uint64_t)t.side_by_side * t.passes && t.blocks() * times > 2 * resident) t.passes *= 2;
         return t;
     }
-    uint64_t blocks(int passes) const {
+    uint64_t blocks() const {
         const uint64_t tile = (uint64_t)side_by_side * passes;
         return (lines + tile - 1) / tile * by_chunks.d;
     }
@@ -85,16 +109,16 @@ struct Lane {
     uint64_t line;  // of the first pass; the next ones are side_by_side further each
     uint64_t unit;  // of the line
     bool in;        // has a unit; lanes without one still take part in a warp's votes and shuffles
-    __device__ __forceinline__ Lane(const Tiling &t, uint32_t block, int passes) {
+    __device__ __forceinline__ Lane(const Tiling &t, uint32_t block) {
         uint32_t chunk, place;
         const uint32_t tile = t.by_chunks.divmod(block, chunk);
         if (t.by_chunks.d == 1) {
             const uint32_t local = t.by_width.divmod(threadIdx.x, place);
-            line = (uint64_t)tile * (t.side_by_side * passes) + local;
+            line = (uint64_t)tile * (t.side_by_side * t.passes) + local;
             unit = place;
             in = local < t.side_by_side;
         } else {
-            line = (uint64_t)tile * passes;
+            line = (uint64_t)tile * t.passes;
             unit = (uint64_t)chunk * t.threads + threadIdx.x;
             in = unit < t.width && threadIdx.x < t.threads;  // a CTA may be wider than this tiling asks for
         }
@@ -130,8 +154,6 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
 }
 
 // ---- wide elements -------------------------------------------------------------------------------------------
-// A unit is V consecutive values of one row held by one lane: 16 (32-byte accesses), 8 (16-byte accesses) or 1 (any
-// alignment).  32 / V neighbouring lanes hold a group.
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -167,7 +189,8 @@ struct Unit {  // as it lies in memory
 #pragma unroll
         for (int i = 0; i < kWords; ++i) w[i] = 0;
     }
-    __device__ __forceinline__ void load(const T *p) {
+    // `left`: columns from the unit's first one to the end of the row; positive, so a whole unit is there
+    __device__ __forceinline__ void load(const T *p, int left) {
         if constexpr (V == 16) {
 #pragma unroll
             for (int i = 0; i < kWords; i += 8)
@@ -182,7 +205,7 @@ struct Unit {  // as it lies in memory
             }
         }
     }
-    __device__ __forceinline__ void store(T *p) const {
+    __device__ __forceinline__ void store(T *p, int left) const {
         if constexpr (V == 16) {
 #pragma unroll
             for (int i = 0; i < kWords; i += 8)
@@ -231,26 +254,42 @@ struct Unit {  // as it lies in memory
 };
 template <typename T>
 struct Unit<T, 1> {
-    T x;
-    __device__ __forceinline__ void clear() { x = from_f32<T>(0.0f); }
-    __device__ __forceinline__ void load(const T *p) { x = *p; }
-    __device__ __forceinline__ void store(T *p) const { *p = x; }
-    __device__ __forceinline__ float value(int) const { return to_f32(x); }
-    __device__ __forceinline__ Pair pair(int) const { return Pair(to_f32(x), 0.0f); }
-    template <bool FINITE>
-    __device__ __forceinline__ void set_pair(int, Pair v) {
-        if constexpr (FINITE && std::is_same_v<T, __half>) x = __ushort_as_half((unsigned short)pair_from_f32<__half, true>(v.get().x, 0.0f));
-        else x = from_f32<T>(v.get().x);
+    T x[kStridedValues];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < kStridedValues; ++j) x[j] = from_f32<T>(0.0f);
     }
-    __device__ __forceinline__ unsigned top_bits() const { return __float_as_uint(fmaxf(0.0f, fabsf(to_f32(x)))); }
+    __device__ __forceinline__ void load(const T *p, int left) {
+#pragma unroll
+        for (int j = 0; j < kStridedValues; ++j)
+            if (j * kGroup < left) x[j] = p[j * kGroup];
+    }
+    __device__ __forceinline__ void store(T *p, int left) const {
+#pragma unroll
+        for (int j = 0; j < kStridedValues; ++j)
+            if (j * kGroup < left) p[j * kGroup] = x[j];
+    }
+    __device__ __forceinline__ float value(int j) const { return to_f32(x[j]); }
+    __device__ __forceinline__ Pair pair(int j) const { return Pair(value(j), value(j + 1)); }
+    template <bool FINITE>
+    __device__ __forceinline__ void set_pair(int j, Pair v) {
+        const float2 f = v.get();
+        if constexpr (sizeof(T) == 4) {
+            x[j] = f.x, x[j + 1] = f.y;
+        } else {
+            const uint32_t w = pair_from_f32<T, FINITE>(f.x, f.y);
+            const unsigned short lo = (unsigned short)w, hi = (unsigned short)(w >> 16);
+            x[j] = *reinterpret_cast<const T *>(&lo), x[j + 1] = *reinterpret_cast<const T *>(&hi);
+        }
+    }
 };
 
 // ---- scales and codes ---------------------------------------------------------------------------------------
-__device__ __forceinline__ int scale_byte(unsigned top_bits) {
+__device__ __forceinline__ unsigned scale_byte(unsigned top_bits) {
     const int b = (int)((top_bits + 0x1fffffu) >> 23) - 8;
-    return min(max(b, 0), kMaxScaleByte);
+    return (unsigned)min(max(b, 0), kMaxScaleByte);
 }
-__device__ __forceinline__ float scale_inverse(int b) { return __uint_as_float((unsigned)(254 - b) << 23); }
+__device__ __forceinline__ float scale_inverse(unsigned b) { return __uint_as_float((254u - b) << 23); }
 // 2^(b - 127); b = 0 is the subnormal 2^-127
 __device__ __forceinline__ float scale_value(unsigned b) { return __uint_as_float(max(b << 23, 0x00400000u)); }
 
@@ -264,15 +303,18 @@ __device__ __forceinline__ float nan_if_infinite(float x) {
     return (__float_as_uint(x) & 0x7fffffffu) == kInfBits ? __uint_as_float(0x7fffffffu) : x;
 }
 
-// largest over the lanes of a group; every lane of the warp calls it
+// Largest over the lanes of a group of 32 / V lanes; every lane of the warp calls it.
 template <int V>
 __device__ __forceinline__ unsigned group_max(unsigned m) {
-    if constexpr (V == 1) return __reduce_max_sync(0xffffffffu, m);
-    else {
 #pragma unroll
-        for (int o = 1; o < kGroup / V; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        return m;
-    }
+    for (int o = 1; o < kGroup / V; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+// bits of the largest |x| of a warp that is not NaN
+__device__ __forceinline__ unsigned warp_top_bits(float x) {
+    float m;
+    asm volatile("redux.sync.max.abs.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
+    return __float_as_uint(fabsf(m));
 }
 
 __device__ __forceinline__ uint16_t to_codes(float lo, float hi) {  // saturates at +-448, NaN -> 0x7f
@@ -282,66 +324,110 @@ __device__ __forceinline__ uint16_t to_codes(float lo, float hi) {  // saturates
 }
 
 template <int V>
-struct Codes {  // of one unit
-    uint32_t w[(V + 3) / 4];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < (V + 3) / 4; ++i) w[i] = 0;
-    }
-    __device__ __forceinline__ void load(const uint8_t *p) {
+struct Codes {  // of one unit, four to a word
+    static constexpr int kWords = Form<V>::kValues / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const uint8_t *p, int left) {
         if constexpr (V == 16) {
             const uint4 v = ld_stream<2>(reinterpret_cast<const uint4 *>(p));
             w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
         } else if constexpr (V == 8) {
             asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
         } else {
-            w[0] = *p;
+            uint32_t c[kStridedValues];
+#pragma unroll
+            for (int j = 0; j < kStridedValues; ++j) c[j] = j * kGroup < left ? p[j * kGroup] : 0u;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = c[4 * i] | c[4 * i + 1] << 8 | c[4 * i + 2] << 16 | c[4 * i + 3] << 24;
         }
     }
-    __device__ __forceinline__ void store(uint8_t *p) const {
+    __device__ __forceinline__ void store(uint8_t *p, int left) const {
         if constexpr (V == 16) st_stream<2>(reinterpret_cast<uint4 *>(p), make_uint4(w[0], w[1], w[2], w[3]));
         else if constexpr (V == 8) asm volatile("st.global.L1::no_allocate.v2.u32 [%0], {%1,%2};" :: "l"(p), "r"(w[0]), "r"(w[1]) : "memory");
-        else *p = (uint8_t)w[0];
+        else {
+#pragma unroll
+            for (int j = 0; j < kStridedValues; ++j)
+                if (j * kGroup < left) p[j * kGroup] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
+        }
     }
     // values j and j + 1 (j even), in 32 bits: a code is an f16 value exactly, and its product with a power of two is exact
-    __device__ __forceinline__ Pair pair(int j, float scale) const {
+    __device__ __forceinline__ Pair pair(int j, Pair scale) const {
         uint32_t r;
         asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)(w[j / 4] >> (8 * (j & 2)))));
         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
-        return Pair(f.x, f.y) * Pair(scale);
+        return Pair(f.x, f.y) * scale;
     }
 };
 
-// Packs a unit: its codes, and the scale byte of its group (the same in all lanes of the group).  Every lane of the warp calls
-// it; lanes without values come with a cleared unit.  The maximum ignores NaN, which convert to the NaN code by
-// themselves; infinities are rare, so only when one is found somewhere in the warp the values are looked at one by one.
+template <int V>
+struct Scales {  // of one unit
+    unsigned b[Form<V>::kScales];
+    __device__ __forceinline__ void load(const uint8_t *p, int left) {
+        if constexpr (V != 1) b[0] = *p;
+        else {
+#pragma unroll
+            for (int j = 0; j < kStridedValues; ++j) b[j] = j * kGroup < left ? p[j] : 0u;
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t *p, int left) const {
+        if constexpr (V != 1) *p = (uint8_t)b[0];
+        else {
+#pragma unroll
+            for (int j = 0; j < kStridedValues; ++j)
+                if (j * kGroup < left) p[j] = (uint8_t)b[j];
+        }
+    }
+    __device__ __forceinline__ Pair pair(int j) const {
+        if constexpr (V != 1) return Pair(scale_value(b[0]));
+        else return Pair(scale_value(b[j]), scale_value(b[j + 1]));
+    }
+};
+
+// Packs a unit.  Every lane of the warp calls it; lanes without values come with a cleared unit.  The maximum ignores NaN, which
+// convert to the NaN code by themselves; infinities are rare, so only when one is found somewhere in the warp the
+// values are looked at one by one.
 template <typename T, int V>
-__device__ __forceinline__ int pack_unit(const Unit<T, V> &in, Codes<V> &out) {
-    float x[V];
+__device__ __forceinline__ void pack_unit(const Unit<T, V> &in, Codes<V> &out, Scales<V> &scales) {
+    constexpr int N = Form<V>::kValues;
+    float x[N];
 #pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = in.value(j);
-    unsigned top = group_max<V>(in.top_bits());
-    if (__any_sync(0xffffffffu, top >= kInfBits)) {
-        top = 0;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            top = max(top, finite_magnitude(x[j]));
-            x[j] = nan_if_infinite(x[j]);
-        }
-        top = group_max<V>(top);
-    }
-    const int b = scale_byte(top);
-    const float inverse = scale_inverse(b);
+    for (int j = 0; j < N; ++j) x[j] = in.value(j);
     if constexpr (V == 1) {
-        out.w[0] = to_codes(x[0] * inverse, 0.0f) & 0xffu;
-    } else {
+        unsigned top[N], most = 0;
 #pragma unroll
-        for (int j = 0; j < V; j += 4) {
-            const float2 lo = (Pair(x[j], x[j + 1]) * Pair(inverse)).get(), hi = (Pair(x[j + 2], x[j + 3]) * Pair(inverse)).get();
-            out.w[j / 4] = (uint32_t)to_codes(lo.x, lo.y) | (uint32_t)to_codes(hi.x, hi.y) << 16;
+        for (int j = 0; j < N; ++j) {
+            top[j] = warp_top_bits(x[j]);
+            most = max(most, top[j]);
         }
+        if (most >= kInfBits) {  // the same in all lanes
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                top[j] = __reduce_max_sync(0xffffffffu, finite_magnitude(x[j]));
+                x[j] = nan_if_infinite(x[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) scales.b[j] = scale_byte(top[j]);
+    } else {
+        unsigned top = group_max<V>(in.top_bits());
+        if (__any_sync(0xffffffffu, top >= kInfBits)) {
+            top = 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                top = max(top, finite_magnitude(x[j]));
+                x[j] = nan_if_infinite(x[j]);
+            }
+            top = group_max<V>(top);
+        }
+        scales.b[0] = scale_byte(top);
     }
-    return b;
+    auto codes = [&](int j) {
+        const Pair inverse(scale_inverse(scales.b[V == 1 ? j : 0]), scale_inverse(scales.b[V == 1 ? j + 1 : 0]));
+        const float2 y = (Pair(x[j], x[j + 1]) * inverse).get();
+        return (uint32_t)to_codes(y.x, y.y);
+    };
+#pragma unroll
+    for (int j = 0; j < N; j += 4) out.w[j / 4] = codes(j) | codes(j + 2) << 16;
 }
 
 // ---- sigmoid --------------------------------------------------------------------------------------------------

@@ -36,23 +36,27 @@ struct Pool {
 // A lane's tokens and its place in their heads.
 template <int V>
 struct Place {
-    uint64_t token, wide;    // wide: offset of the lane's values from the token's
-    uint64_t code, scale;    // the same in the pool
-    uint32_t step;
-    bool in_row, leads, first;
+    uint64_t token, wide;  // wide: offset of the lane's values from the token's
+    uint64_t code, scale;  // the same in the pool
+    uint32_t step, passes;
+    int left, scales_left;  // columns from the unit's first one, and from its groups' first one, on; 0: no unit
+    bool leads, first;
     template <typename T>
     __device__ __forceinline__ Place(const Side<T> &s, uint32_t block) {
-        const Lane lane(s.tiling, block, kPasses);
+        const Lane lane(s.tiling, block);
         token = lane.line;
         step = s.tiling.side_by_side;
+        passes = s.tiling.passes;
         uint32_t unit;
         const uint32_t head = s.per_row.divmod((uint32_t)lane.unit, unit);
+        const uint32_t column = (uint32_t)Form<V>::column(unit);
         const uint64_t row = (uint64_t)head * s.head_rows;
-        wide = head * s.head_stride + unit * V;
-        code = row * s.dim + unit * V;
-        scale = row * s.groups + unit / (kGroup / V);
-        in_row = lane.in && unit * V < s.dim;
-        leads = (unit & (kGroup / V - 1)) == 0;
+        wide = head * s.head_stride + column;
+        code = row * s.dim + column;
+        scale = row * s.groups + Form<V>::scale(unit);
+        left = lane.in && column < s.dim ? (int)(s.dim - column) : 0;
+        scales_left = V == 1 ? left + (int)(column % kGroup) : left;
+        leads = Form<V>::leads(unit);
         first = lane.unit == 0;
     }
 };
@@ -75,15 +79,17 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
         const uint64_t token = at.token + u * at.step;
         slot[u] = -1;
         x[u].clear();
-        if (at.in_row && token < tokens) {
+        if (u < at.passes && at.left > 0 && token < tokens) {
             slot[u] = slots[token];
-            x[u].load(from + u * (at.step * s.token_stride));
+            x[u].load(from + u * (at.step * s.token_stride), at.left);
         }
     }
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
+        if (u >= at.passes) break;
         Codes<V> c;
-        const int b = pack_unit(x[u], c);
+        Scales<V> b;
+        pack_unit(x[u], c, b);
         if (slot[u] < 0) continue;
         if ((uint64_t)slot[u] >= pool.slots) {
             if (at.first) raise_error(errors, kErrIndexRange);
@@ -95,8 +101,8 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
             row = pool.page_tokens.divmod((uint64_t)slot[u], offset) * pool.page_rows;
             row += offset;
         }
-        c.store(s.codes + row * s.dim + at.code);
-        if (at.leads) s.scales[row * s.groups + at.scale] = (uint8_t)b;
+        c.store(s.codes + row * s.dim + at.code, at.left);
+        if (at.leads) b.store(s.scales + row * s.groups + at.scale, at.scales_left);
     }
 }
 
@@ -127,27 +133,27 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
     for (int u = 0; u < kPasses; ++u) {
         const uint32_t p = (uint32_t)at.token + u * at.step;
         const uint32_t entry = pool.page_tokens32.divmod(p, offset[u]);
-        page[u] = p < q.max_length ? table[entry] : 0;
+        page[u] = u < at.passes && p < q.max_length ? table[entry] : 0;
     }
     if (block == 0 && threadIdx.x == 0 && (length < 0 || (uint32_t)length > q.max_length)) raise_error(errors, kErrIndexRange);
     const uint32_t n = length < 0 ? 0 : min((uint32_t)length, q.max_length);
     const int64_t row = first_row + (int64_t)at.token;
     T *to = s.wide + (uint64_t)row * s.token_stride + at.wide;  // not formed into an access before its row is checked
     Codes<V> c[kPasses];
-    unsigned scale[kPasses];
+    Scales<V> scale[kPasses];
     bool live[kPasses];
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
         const uint32_t p = (uint32_t)at.token + u * at.step;
-        live[u] = at.in_row && p < n;
+        live[u] = u < at.passes && at.left > 0 && p < n;
         if (live[u] && ((uint32_t)page[u] >= pool.pages || (uint64_t)(row + (int64_t)(u * at.step)) >= q.rows)) {
             if (at.first) raise_error(errors, kErrIndexRange);
             live[u] = false;
         }
         if (live[u]) {
             const uint64_t from = (uint32_t)page[u] * pool.page_rows + (uint64_t)offset[u] * s.token_rows;
-            c[u].load(s.codes + from * s.dim + at.code);
-            scale[u] = s.scales[from * s.groups + at.scale];
+            c[u].load(s.codes + from * s.dim + at.code, at.left);
+            scale[u].load(s.scales + from * s.groups + at.scale, at.scales_left);
         }
     }
 #pragma unroll
@@ -155,8 +161,8 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
         if (!live[u]) continue;
         Unit<T, V> y;
 #pragma unroll
-        for (int j = 0; j < V; j += 2) y.template set_pair<true>(j, c[u].pair(j, scale_value(scale[u])));
-        y.store(to + u * (at.step * s.token_stride));
+        for (int j = 0; j < Form<V>::kValues; j += 2) y.template set_pair<true>(j, c[u].pair(j, scale[u].pair(j)));
+        y.store(to + u * (at.step * s.token_stride), at.left);
     }
 }
 
@@ -182,17 +188,18 @@ struct Wide {  // the wide tensor of a side, as given
 // Keys and values go to one launch where their units are the same, else to one each.
 // launch(v, k side, v side): either side may have no blocks.
 template <typename T, typename Launch>
-int by_sides(const lcbCacheQ8 &c, const Wide &k, const Wide &v, size_t tokens, size_t rows, Launch launch) {
+int by_sides(const lcbCacheQ8 &c, const Wide &k, const Wide &v, size_t tokens, size_t rows, size_t sequences, Launch launch) {
     const int ku = k.unit(c, rows, sizeof(T)), vu = c.v_dim != 0 ? v.unit(c, rows, sizeof(T)) : ku;
     auto side = [&](const Wide &w, int unit, bool on) {
         Side<T> s{};
         if (!on || w.dim == 0) return s;
-        const uint64_t groups = groups_of(w.dim), per_row = groups * (kGroup / unit);
+        const uint64_t groups = groups_of(w.dim);
+        const uint64_t per_row = unit == 16 ? Form<16>::per_row(groups) : unit == 8 ? Form<8>::per_row(groups) : Form<1>::per_row(groups);
         const bool heads_first = c.order == LCB_CACHE_HEADS_FIRST;
         s = {static_cast<T *>(const_cast<void *>(w.p)), w.token_stride, w.head_stride, static_cast<uint8_t *>(w.codes), static_cast<uint8_t *>(w.scales),
              (uint32_t)w.dim, (uint32_t)groups, heads_first ? 1u : (uint32_t)c.heads, heads_first ? (uint32_t)c.page_tokens : 1u,
-             FastDiv32::of((uint32_t)per_row), Tiling::of(tokens, c.heads * per_row), 0};
-        s.blocks = (uint32_t)std::min<uint64_t>(s.tiling.blocks(kPasses), 0x80000000u);  // too many: refused by the launch
+             FastDiv32::of((uint32_t)per_row), Tiling::of(tokens, c.heads * per_row, kPasses, 2 * sequences), 0};
+        s.blocks = (uint32_t)std::min<uint64_t>(s.tiling.blocks(), 0x80000000u);  // too many: refused by the launch
         return s;
     };
     const bool both = ku == vu;
@@ -223,7 +230,7 @@ extern "C" int lcb_cache_write_q8(const lcbCacheQ8 *cache, const void *k, size_t
     const Wide vw{v, v_token_stride, v_head_stride, cache->v_dim, cache->v_codes, cache->v_scales};
     return with_type(type, [&](auto *t) {
         using T = const std::remove_pointer_t<decltype(t)>;
-        return by_sides<T>(*cache, kw, vw, tokens, tokens, [&](auto u, const Side<T> &ks, const Side<T> &vs) {
+        return by_sides<T>(*cache, kw, vw, tokens, tokens, 1, [&](auto u, const Side<T> &ks, const Side<T> &vs) {
             const uint64_t blocks = (uint64_t)ks.blocks + vs.blocks;
             if (blocks > 0x7fffffffu) return 1;
             const unsigned threads = std::max(ks.tiling.threads, vs.tiling.threads);
@@ -247,7 +254,7 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
     const Wide vw{v, v_token_stride, v_head_stride, cache->v_dim, cache->v_codes, cache->v_scales};
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return by_sides<T>(*cache, kw, vw, max_length, rows, [&](auto u, const Side<T> &ks, const Side<T> &vs) {
+        return by_sides<T>(*cache, kw, vw, max_length, rows, sequences, [&](auto u, const Side<T> &ks, const Side<T> &vs) {
             const uint64_t each = (uint64_t)ks.blocks + vs.blocks;
             if (each > 0x7fffffffu || sequences > 0x7fffffffu / each) return 1;
             const Sequences q{page_table, lengths, first_rows, table_stride, rows, (uint32_t)max_length, FastDiv32::of((uint32_t)each)};

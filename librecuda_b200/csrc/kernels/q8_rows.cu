@@ -9,9 +9,11 @@
 namespace lcb {
 namespace {
 
-constexpr int kPasses = 4;      // units in flight per lane: pack, unpack
-constexpr int kPassesSilu = 2;  // the gated unit holds two inputs
-constexpr int kPassesGrad = 1;  // and its gradient three, with three outputs
+// units in flight per lane, at most
+constexpr int kPasses = 4;
+constexpr int kPassesUnpack = 2;
+constexpr int kPassesSilu = 2;  // of each input
+constexpr int kPassesGrad = 1;
 
 template <typename T>
 struct Rows {  // rows of the wide type
@@ -25,84 +27,92 @@ struct Packed {
 struct Shape {
     uint64_t rows, cols, groups;
     Tiling tiling;
-    static Shape of(size_t rows, size_t cols, int v) {
+    template <int V>
+    static Shape of(size_t rows, size_t cols, int max_passes) {
         const uint64_t groups = groups_of(cols);
-        return {rows, cols, groups, Tiling::of(rows, groups * (kGroup / v))};
+        return {rows, cols, groups, Tiling::of(rows, Form<V>::per_row(groups), max_passes)};
     }
 };
 
-// A lane's column and its rows.  The columns of a unit are all inside the matrix or all behind it; lanes behind the last
-// column of a row still belong to its last group.
+// A lane's column and its rows.
 template <int V>
 struct Place {
-    uint64_t row, unit, left;  // left: rows from `row` on
-    uint32_t step;
-    bool in_row;
-    __device__ __forceinline__ Place(const Shape &s, int passes) {
-        const Lane lane(s.tiling, blockIdx.x, passes);
+    uint64_t row, column, first_scale;
+    uint64_t rows_left;  // from `row` on
+    uint32_t step, passes;
+    int left;  // columns from the unit's first one on; 0 where it lies behind the row (V > 1: a row ends with a whole unit)
+    bool leads;
+    __device__ __forceinline__ explicit Place(const Shape &s) {
+        const Lane lane(s.tiling, blockIdx.x);
         row = lane.line;
-        unit = lane.unit;
+        column = Form<V>::column(lane.unit);
+        first_scale = Form<V>::scale(lane.unit);
+        leads = Form<V>::leads(lane.unit);
         step = s.tiling.side_by_side;
-        in_row = lane.in && unit * V < s.cols && row < s.rows;
-        left = s.rows - row;
+        passes = s.tiling.passes;
+        left = lane.in && column < s.cols ? (int)min(s.cols - column, (uint64_t)INT32_MAX) : 0;
+        rows_left = row < s.rows ? s.rows - row : 0;
     }
-    __device__ __forceinline__ bool in(int pass) const { return in_row && pass * step < left; }
-    __device__ __forceinline__ bool leads() const { return (unit & (kGroup / V - 1)) == 0; }
+    __device__ __forceinline__ bool in(int pass) const { return left > 0 && pass * step < rows_left; }
     __device__ __forceinline__ uint8_t *code(const Packed &p, const Shape &s, int pass) const {
-        return p.codes + (row * s.cols + unit * V) + pass * (step * s.cols);
+        return p.codes + (row * s.cols + column) + pass * (step * s.cols);
     }
     __device__ __forceinline__ uint8_t *scale(const Packed &p, const Shape &s, int pass) const {
-        return p.scales + (row * s.groups + unit / (kGroup / V)) + pass * (step * s.groups);
+        return p.scales + (row * s.groups + first_scale) + pass * (step * s.groups);
     }
+    // columns from the first value of the unit's groups on: what decides which scales there are
+    __device__ __forceinline__ int scales_left(const Shape &s) const { return V == 1 ? left + (int)(column % kGroup) : left; }
     template <typename T>
-    __device__ __forceinline__ T *wide(const Rows<T> &r, int pass) const { return r.p + (row * r.stride + unit * V) + pass * (step * r.stride); }
+    __device__ __forceinline__ T *wide(const Rows<T> &r, int pass) const { return r.p + (row * r.stride + column) + pass * (step * r.stride); }
 };
 
 template <typename T, int V>
 __device__ __forceinline__ void pack_and_store(const Packed &out, const Shape &s, const Place<V> &at, int pass, const Unit<T, V> &x) {
     Codes<V> c;
-    const int b = pack_unit(x, c);
+    Scales<V> b;
+    pack_unit(x, c, b);
     if (!at.in(pass)) return;
-    c.store(at.code(out, s, pass));
-    if (at.leads()) *at.scale(out, s, pass) = (uint8_t)b;
+    c.store(at.code(out, s, pass), at.left);
+    if (at.leads) b.store(at.scale(out, s, pass), at.scales_left(s));
 }
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kMaxThreads) pack_kernel(Packed out, Rows<const T> src, Shape s) {
     pdl_launch_dependents();
-    const Place<V> at(s, kPasses);
+    const Place<V> at(s);
     Unit<T, V> x[kPasses];
     pdl_wait();
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
         x[u].clear();
-        if (at.in(u)) x[u].load(at.wide(src, u));
+        if (u < at.passes && at.in(u)) x[u].load(at.wide(src, u), at.left);
     }
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) pack_and_store(out, s, at, u, x[u]);
+    for (int u = 0; u < kPasses; ++u)
+        if (u < at.passes) pack_and_store(out, s, at, u, x[u]);
 }
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kMaxThreads) unpack_kernel(Rows<T> dst, Packed in, Shape s) {
     pdl_launch_dependents();
-    const Place<V> at(s, kPasses);
-    Codes<V> c[kPasses];
-    unsigned b[kPasses];
+    const Place<V> at(s);
+    Codes<V> c[kPassesUnpack];
+    Scales<V> b[kPassesUnpack];
     pdl_wait();
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-        if (at.in(u)) {
-            c[u].load(at.code(in, s, u));
-            b[u] = *at.scale(in, s, u);
+    for (int u = 0; u < kPassesUnpack; ++u) {
+        if (u < at.passes && at.in(u)) {
+            c[u].load(at.code(in, s, u), at.left);
+            b[u].load(at.scale(in, s, u), at.scales_left(s));
         }
     }
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-        if (!at.in(u)) continue;
+    for (int u = 0; u < kPassesUnpack; ++u) {
+        if (u >= at.passes || !at.in(u)) continue;
         Unit<T, V> y;
 #pragma unroll
-        for (int j = 0; j < V; j += 2) y.template set_pair<true>(j, c[u].pair(j, scale_value(b[u])));
-        y.store(at.wide(dst, u));
+        for (int j = 0; j < Form<V>::kValues; j += 2) y.template set_pair<true>(j, c[u].pair(j, b[u].pair(j)));
+        y.store(at.wide(dst, u), at.left);
     }
 }
 
@@ -110,28 +120,29 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kMaxThreads) silu_mul_pack_kernel(Rows<T> h, Packed gate_out, Packed up_out, Rows<const T> gate,
                                                                     Rows<const T> up, Shape s) {
     pdl_launch_dependents();
-    const Place<V> at(s, kPassesSilu);
+    const Place<V> at(s);
     Unit<T, V> g[kPassesSilu], u[kPassesSilu];
     pdl_wait();
 #pragma unroll
     for (int k = 0; k < kPassesSilu; ++k) {
         g[k].clear();
         u[k].clear();
-        if (at.in(k)) {
-            g[k].load(at.wide(gate, k));
-            u[k].load(at.wide(up, k));
+        if (k < at.passes && at.in(k)) {
+            g[k].load(at.wide(gate, k), at.left);
+            u[k].load(at.wide(up, k), at.left);
         }
     }
 #pragma unroll
     for (int k = 0; k < kPassesSilu; ++k) {
+        if (k >= at.passes) break;
         if (at.in(k)) {
             Unit<T, V> out;
 #pragma unroll
-            for (int j = 0; j < V; j += 2) {
+            for (int j = 0; j < Form<V>::kValues; j += 2) {
                 const Pair x = g[k].pair(j);
                 out.template set_pair<false>(j, x * sigmoid(x).s * u[k].pair(j));
             }
-            out.store(at.wide(h, k));
+            out.store(at.wide(h, k), at.left);
         }
         pack_and_store(gate_out, s, at, k, g[k]);
         pack_and_store(up_out, s, at, k, u[k]);
@@ -142,39 +153,31 @@ template <typename T, int V, bool AGAIN>
 __global__ void __launch_bounds__(kMaxThreads) silu_mul_grad_kernel(Rows<T> dgate, Rows<T> dup, Rows<T> h, Rows<const T> dh, Packed gate,
                                                                     Packed up, Shape s) {
     pdl_launch_dependents();
-    const Place<V> at(s, kPassesGrad);
-    Unit<T, V> d[kPassesGrad];
-    Codes<V> g[kPassesGrad], u[kPassesGrad];
-    unsigned gb[kPassesGrad], ub[kPassesGrad];
+    const Place<V> at(s);
     pdl_wait();
+    if (!at.in(0)) return;
+    Unit<T, V> d;
+    Codes<V> g, u;
+    Scales<V> gs, us;
+    d.clear();
+    d.load(at.wide(dh, 0), at.left);
+    g.load(at.code(gate, s, 0), at.left);
+    u.load(at.code(up, s, 0), at.left);
+    gs.load(at.scale(gate, s, 0), at.scales_left(s));
+    us.load(at.scale(up, s, 0), at.scales_left(s));
+    Unit<T, V> dg, du, y;
 #pragma unroll
-    for (int k = 0; k < kPassesGrad; ++k) {
-        if (at.in(k)) {
-            d[k].load(at.wide(dh, k));
-            g[k].load(at.code(gate, s, k));
-            u[k].load(at.code(up, s, k));
-            gb[k] = *at.scale(gate, s, k);
-            ub[k] = *at.scale(up, s, k);
-        }
+    for (int j = 0; j < Form<V>::kValues; j += 2) {
+        const Pair x = g.pair(j, gs.pair(j)), z = u.pair(j, us.pair(j)), dj = d.pair(j);
+        const Sigmoid sg = sigmoid(x);
+        const Pair silu = x * sg.s;
+        du.template set_pair<false>(j, dj * silu);
+        dg.template set_pair<false>(j, dj * z * fma2(silu, sg.q, sg.s));
+        if constexpr (AGAIN) y.template set_pair<false>(j, silu * z);
     }
-#pragma unroll
-    for (int k = 0; k < kPassesGrad; ++k) {
-        if (!at.in(k)) continue;
-        const float gs = scale_value(gb[k]), us = scale_value(ub[k]);
-        Unit<T, V> dg, du, y;
-#pragma unroll
-        for (int j = 0; j < V; j += 2) {
-            const Pair x = g[k].pair(j, gs), z = u[k].pair(j, us), dj = d[k].pair(j);
-            const Sigmoid sg = sigmoid(x);
-            const Pair silu = x * sg.s;
-            du.template set_pair<false>(j, dj * silu);
-            dg.template set_pair<false>(j, dj * z * fma2(silu, sg.q, sg.s));
-            if constexpr (AGAIN) y.template set_pair<false>(j, silu * z);
-        }
-        du.store(at.wide(dup, k));
-        dg.store(at.wide(dgate, k));
-        if constexpr (AGAIN) y.store(at.wide(h, k));
-    }
+    du.store(at.wide(dup, 0), at.left);
+    dg.store(at.wide(dgate, 0), at.left);
+    if constexpr (AGAIN) y.store(at.wide(h, 0), at.left);
 }
 
 // The widest unit whose accesses are aligned in every row: codes and values of a unit start at multiples of its size.
@@ -195,8 +198,8 @@ struct Fit {
 };
 
 template <typename... KArgs, typename... Args>
-int launch_rows(void (*kernel)(KArgs...), int passes, const Shape &s, lcbStream stream, Args... args) {
-    const uint64_t blocks = s.tiling.blocks(passes);
+int launch_rows(void (*kernel)(KArgs...), const Shape &s, lcbStream stream, Args... args) {
+    const uint64_t blocks = s.tiling.blocks();
     if (blocks > 0x7fffffffu) return 1;
     return launch_kernel(kernel, (unsigned)blocks, s.tiling.threads, 0, static_cast<cudaStream_t>(stream), args..., s);
 }
@@ -224,7 +227,7 @@ extern "C" int lcb_pack_q8(void *codes, void *scales, const void *src, size_t sr
         fit.add(in, rows);
         fit.add(out);
         return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(pack_kernel<T, v()>, kPasses, Shape::of(rows, cols, v()), stream, out, in);
+            return launch_rows(pack_kernel<T, v()>, Shape::of<v()>(rows, cols, kPasses), stream, out, in);
         });
     });
 }
@@ -241,7 +244,7 @@ extern "C" int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void 
         fit.add(out, rows);
         fit.add(in);
         return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(unpack_kernel<T, v()>, kPasses, Shape::of(rows, cols, v()), stream, out, in);
+            return launch_rows(unpack_kernel<T, v()>, Shape::of<v()>(rows, cols, kPassesUnpack), stream, out, in);
         });
     });
 }
@@ -263,7 +266,7 @@ extern "C" int lcb_silu_mul_pack_q8(void *h, size_t h_stride, void *gate_codes, 
         fit.add(gp);
         fit.add(upk);
         return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(silu_mul_pack_kernel<T, v()>, kPassesSilu, Shape::of(rows, cols, v()), stream, out, gp, upk, g, u);
+            return launch_rows(silu_mul_pack_kernel<T, v()>, Shape::of<v()>(rows, cols, kPassesSilu), stream, out, gp, upk, g, u);
         });
     });
 }
@@ -288,8 +291,8 @@ extern "C" int lcb_silu_mul_grad_q8(void *dgate, size_t dgate_stride, void *dup,
         fit.add(gp);
         fit.add(upk);
         return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(h != nullptr ? silu_mul_grad_kernel<T, v(), true> : silu_mul_grad_kernel<T, v(), false>, kPassesGrad,
-                               Shape::of(rows, cols, v()), stream, dg, du, out, d, gp, upk);
+            return launch_rows(h != nullptr ? silu_mul_grad_kernel<T, v(), true> : silu_mul_grad_kernel<T, v(), false>,
+                               Shape::of<v()>(rows, cols, kPassesGrad), stream, dg, du, out, d, gp, upk);
         });
     });
 }
