@@ -52,24 +52,14 @@ struct FastDiv32 {
 };
 
 // ---- units --------------------------------------------------------------------------------------------------------
-// A unit is what one lane holds of a row, in one of three forms V.  V = 16 or 8: that many consecutive values, moved by 32- or
-// 16-byte accesses of the wide type; 32 / V neighbouring lanes hold a group.  V = 1, for rows at any alignment: eight
-// values 32 columns apart, so that a warp holds eight groups, each access of the warp covers the values of one group side
-// by side, and the maximum of a group is one warp-wide instruction.
-constexpr int kStridedValues = 8;
+// A unit is kValues consecutive values of a row, held by one lane; kLanes neighbouring lanes hold a group.  Three forms V:
+// 16 values in 32-byte accesses of the wide type, 8 in 16-byte ones, and, as V = 1, 8 values at any address, whose row may
+// end inside the unit.
 template <int V>
 struct Form {
-    static constexpr int kValues = V == 1 ? kStridedValues : V;
-    static constexpr int kScales = V == 1 ? kStridedValues : 1;  // groups that a unit has a part of
-    static constexpr int kLanes = kGroup / V;                    // lanes that share them
-    __host__ __device__ static uint64_t per_row(uint64_t groups) {
-        return V == 1 ? (groups + kStridedValues - 1) / kStridedValues * kGroup : groups * kLanes;
-    }
-    __device__ static __forceinline__ uint64_t column(uint64_t unit) {
-        return V == 1 ? unit / kGroup * (kGroup * kStridedValues) + unit % kGroup : unit * V;
-    }
-    __device__ static __forceinline__ uint64_t scale(uint64_t unit) { return V == 1 ? unit / kGroup * kStridedValues : unit / kLanes; }
-    __device__ static __forceinline__ bool leads(uint64_t unit) { return unit % kLanes == 0; }  // writes the scales
+    static constexpr int kValues = V == 1 ? 8 : V;
+    static constexpr int kLanes = kGroup / kValues;
+    __host__ __device__ static uint64_t per_row(uint64_t groups) { return groups * kLanes; }
 };
 
 // ---- which units a lane works on --------------------------------------------------------------------------------
@@ -183,13 +173,14 @@ __device__ __forceinline__ uint32_t pair_from_f32(float lo, float hi) {
 
 template <typename T, int V>
 struct Unit {  // as it lies in memory
-    static constexpr int kWords = V * (int)sizeof(T) / 4;
+    static constexpr int kValues = Form<V>::kValues;
+    static constexpr int kWords = kValues * (int)sizeof(T) / 4;
     uint32_t w[kWords];
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) w[i] = 0;
     }
-    // `left`: columns from the unit's first one to the end of the row; positive, so a whole unit is there
+    // `left` > 0: columns from the unit's first one to the end of the row.  Values behind the end are 0.
     __device__ __forceinline__ void load(const T *p, int left) {
         if constexpr (V == 16) {
 #pragma unroll
@@ -197,11 +188,28 @@ struct Unit {  // as it lies in memory
                 asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                              : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
                              : "l"(reinterpret_cast<const uint32_t *>(p) + i));
-        } else {
+        } else if constexpr (V == 8) {
 #pragma unroll
             for (int i = 0; i < kWords; i += 4) {
                 const uint4 v = ld_stream<2>(reinterpret_cast<const uint4 *>(p) + i / 4);
                 w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+            }
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = i < left ? reinterpret_cast<const uint32_t *>(p)[i] : 0u;
+        } else {
+            // the aligned words that hold at least one of the values, shifted by half a word where the address asks for it
+            const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(p) >> 1) & 1u;
+            const uint32_t *q = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+            const int n = min(left, kValues) + (int)odd;
+            uint32_t r[kWords + 1];
+#pragma unroll
+            for (int i = 0; i <= kWords; ++i) r[i] = 2 * i < n ? q[i] : 0u;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(r[i], r[i + 1], 16 * odd);
+            if (left < kValues) {
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) w[i] = 2 * i + 1 < left ? w[i] : 2 * i < left ? w[i] & 0xffffu : 0u;
             }
         }
     }
@@ -212,10 +220,29 @@ struct Unit {  // as it lies in memory
                 asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                              :: "l"(reinterpret_cast<uint32_t *>(p) + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
                                 "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7]) : "memory");
-        } else {
+        } else if constexpr (V == 8) {
 #pragma unroll
             for (int i = 0; i < kWords; i += 4)
                 st_stream<2>(reinterpret_cast<uint4 *>(p) + i / 4, make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                if (i < left) reinterpret_cast<uint32_t *>(p)[i] = w[i];
+        } else {
+            uint16_t *h = reinterpret_cast<uint16_t *>(p);
+            if (left < kValues) {
+#pragma unroll
+                for (int j = 0; j < kValues; ++j)
+                    if (j < left) h[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+            } else if ((reinterpret_cast<uintptr_t>(p) & 2) == 0) {
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) reinterpret_cast<uint32_t *>(p)[i] = w[i];
+            } else {
+                h[0] = (uint16_t)w[0];
+#pragma unroll
+                for (int i = 0; i + 1 < kWords; ++i) *reinterpret_cast<uint32_t *>(h + 1 + 2 * i) = __funnelshift_r(w[i], w[i + 1], 16);
+                h[kValues - 1] = (uint16_t)(w[kWords - 1] >> 16);
+            }
         }
     }
     __device__ __forceinline__ float value(int j) const {
@@ -252,38 +279,6 @@ struct Unit {  // as it lies in memory
         }
     }
 };
-template <typename T>
-struct Unit<T, 1> {
-    T x[kStridedValues];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int j = 0; j < kStridedValues; ++j) x[j] = from_f32<T>(0.0f);
-    }
-    __device__ __forceinline__ void load(const T *p, int left) {
-#pragma unroll
-        for (int j = 0; j < kStridedValues; ++j)
-            if (j * kGroup < left) x[j] = p[j * kGroup];
-    }
-    __device__ __forceinline__ void store(T *p, int left) const {
-#pragma unroll
-        for (int j = 0; j < kStridedValues; ++j)
-            if (j * kGroup < left) p[j * kGroup] = x[j];
-    }
-    __device__ __forceinline__ float value(int j) const { return to_f32(x[j]); }
-    __device__ __forceinline__ Pair pair(int j) const { return Pair(value(j), value(j + 1)); }
-    template <bool FINITE>
-    __device__ __forceinline__ void set_pair(int j, Pair v) {
-        const float2 f = v.get();
-        if constexpr (sizeof(T) == 4) {
-            x[j] = f.x, x[j + 1] = f.y;
-        } else {
-            const uint32_t w = pair_from_f32<T, FINITE>(f.x, f.y);
-            const unsigned short lo = (unsigned short)w, hi = (unsigned short)(w >> 16);
-            x[j] = *reinterpret_cast<const T *>(&lo), x[j + 1] = *reinterpret_cast<const T *>(&hi);
-        }
-    }
-};
-
 // ---- scales and codes ---------------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned scale_byte(unsigned top_bits) {
     const int b = (int)((top_bits + 0x1fffffu) >> 23) - 8;
@@ -303,18 +298,12 @@ __device__ __forceinline__ float nan_if_infinite(float x) {
     return (__float_as_uint(x) & 0x7fffffffu) == kInfBits ? __uint_as_float(0x7fffffffu) : x;
 }
 
-// Largest over the lanes of a group of 32 / V lanes; every lane of the warp calls it.
+// Largest over the lanes of a group; every lane of the warp calls it.
 template <int V>
 __device__ __forceinline__ unsigned group_max(unsigned m) {
 #pragma unroll
-    for (int o = 1; o < kGroup / V; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = 1; o < Form<V>::kLanes; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     return m;
-}
-// bits of the largest |x| of a warp that is not NaN
-__device__ __forceinline__ unsigned warp_top_bits(float x) {
-    float m;
-    asm volatile("redux.sync.max.abs.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
-    return __float_as_uint(fabsf(m));
 }
 
 __device__ __forceinline__ uint16_t to_codes(float lo, float hi) {  // saturates at +-448, NaN -> 0x7f
@@ -325,8 +314,8 @@ __device__ __forceinline__ uint16_t to_codes(float lo, float hi) {  // saturates
 
 template <int V>
 struct Codes {  // of one unit, four to a word
-    static constexpr int kWords = Form<V>::kValues / 4;
-    uint32_t w[kWords];
+    static constexpr int kValues = Form<V>::kValues;
+    uint32_t w[kValues / 4];
     __device__ __forceinline__ void load(const uint8_t *p, int left) {
         if constexpr (V == 16) {
             const uint4 v = ld_stream<2>(reinterpret_cast<const uint4 *>(p));
@@ -334,20 +323,45 @@ struct Codes {  // of one unit, four to a word
         } else if constexpr (V == 8) {
             asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
         } else {
-            uint32_t c[kStridedValues];
+            // the aligned words that hold at least one of the codes; codes behind the row's end are whatever lies there
+            const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3);
+            const uint32_t *q = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+            const int n = min(left, kValues) + (int)shift;
+            uint32_t r[3];
 #pragma unroll
-            for (int j = 0; j < kStridedValues; ++j) c[j] = j * kGroup < left ? p[j * kGroup] : 0u;
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) w[i] = c[4 * i] | c[4 * i + 1] << 8 | c[4 * i + 2] << 16 | c[4 * i + 3] << 24;
+            for (int i = 0; i < 3; ++i) r[i] = 4 * i < n ? q[i] : 0u;
+            w[0] = __funnelshift_r(r[0], r[1], 8 * shift);
+            w[1] = __funnelshift_r(r[1], r[2], 8 * shift);
         }
     }
     __device__ __forceinline__ void store(uint8_t *p, int left) const {
         if constexpr (V == 16) st_stream<2>(reinterpret_cast<uint4 *>(p), make_uint4(w[0], w[1], w[2], w[3]));
         else if constexpr (V == 8) asm volatile("st.global.L1::no_allocate.v2.u32 [%0], {%1,%2};" :: "l"(p), "r"(w[0]), "r"(w[1]) : "memory");
-        else {
+        else if (left < kValues) {
 #pragma unroll
-            for (int j = 0; j < kStridedValues; ++j)
-                if (j * kGroup < left) p[j * kGroup] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
+            for (int j = 0; j < kValues; ++j)
+                if (j < left) p[j] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
+        } else {
+            // the widest accesses that the address allows: 1, 2 and 4 bytes in some order
+            const uint32_t m = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3);
+            if (m == 0) {
+                reinterpret_cast<uint32_t *>(p)[0] = w[0];
+                reinterpret_cast<uint32_t *>(p)[1] = w[1];
+            } else if (m == 2) {
+                *reinterpret_cast<uint16_t *>(p) = (uint16_t)w[0];
+                *reinterpret_cast<uint32_t *>(p + 2) = __funnelshift_r(w[0], w[1], 16);
+                *reinterpret_cast<uint16_t *>(p + 6) = (uint16_t)(w[1] >> 16);
+            } else {
+                p[0] = (uint8_t)w[0];
+                if (m == 1) {
+                    *reinterpret_cast<uint16_t *>(p + 1) = (uint16_t)(w[0] >> 8);
+                    *reinterpret_cast<uint32_t *>(p + 3) = __funnelshift_r(w[0], w[1], 24);
+                } else {
+                    *reinterpret_cast<uint32_t *>(p + 1) = __funnelshift_r(w[0], w[1], 8);
+                    *reinterpret_cast<uint16_t *>(p + 5) = (uint16_t)(w[1] >> 8);
+                }
+                p[7] = (uint8_t)(w[1] >> 24);
+            }
         }
     }
     // values j and j + 1 (j even), in 32 bits: a code is an f16 value exactly, and its product with a power of two is exact
@@ -359,75 +373,34 @@ struct Codes {  // of one unit, four to a word
     }
 };
 
-template <int V>
-struct Scales {  // of one unit
-    unsigned b[Form<V>::kScales];
-    __device__ __forceinline__ void load(const uint8_t *p, int left) {
-        if constexpr (V != 1) b[0] = *p;
-        else {
-#pragma unroll
-            for (int j = 0; j < kStridedValues; ++j) b[j] = j * kGroup < left ? p[j] : 0u;
-        }
-    }
-    __device__ __forceinline__ void store(uint8_t *p, int left) const {
-        if constexpr (V != 1) *p = (uint8_t)b[0];
-        else {
-#pragma unroll
-            for (int j = 0; j < kStridedValues; ++j)
-                if (j * kGroup < left) p[j] = (uint8_t)b[j];
-        }
-    }
-    __device__ __forceinline__ Pair pair(int j) const {
-        if constexpr (V != 1) return Pair(scale_value(b[0]));
-        else return Pair(scale_value(b[j]), scale_value(b[j + 1]));
-    }
-};
-
-// Packs a unit.  Every lane of the warp calls it; lanes without values come with a cleared unit.  The maximum ignores NaN, which
-// convert to the NaN code by themselves; infinities are rare, so only when one is found somewhere in the warp the
-// values are looked at one by one.
+// Packs a unit; returns the scale byte of its group.  Every lane of the warp calls it; lanes without values come with a
+// cleared unit.  The maximum ignores NaN, which convert to the NaN code by themselves; infinities are rare, so only when one
+// is found somewhere in the warp the values are looked at one by one.
 template <typename T, int V>
-__device__ __forceinline__ void pack_unit(const Unit<T, V> &in, Codes<V> &out, Scales<V> &scales) {
+__device__ __forceinline__ unsigned pack_unit(const Unit<T, V> &in, Codes<V> &out) {
     constexpr int N = Form<V>::kValues;
     float x[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = in.value(j);
-    if constexpr (V == 1) {
-        unsigned top[N], most = 0;
+    unsigned top = group_max<V>(in.top_bits());
+    if (__any_sync(0xffffffffu, top >= kInfBits)) {
+        top = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            top[j] = warp_top_bits(x[j]);
-            most = max(most, top[j]);
+            top = max(top, finite_magnitude(x[j]));
+            x[j] = nan_if_infinite(x[j]);
         }
-        if (most >= kInfBits) {  // the same in all lanes
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                top[j] = __reduce_max_sync(0xffffffffu, finite_magnitude(x[j]));
-                x[j] = nan_if_infinite(x[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) scales.b[j] = scale_byte(top[j]);
-    } else {
-        unsigned top = group_max<V>(in.top_bits());
-        if (__any_sync(0xffffffffu, top >= kInfBits)) {
-            top = 0;
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                top = max(top, finite_magnitude(x[j]));
-                x[j] = nan_if_infinite(x[j]);
-            }
-            top = group_max<V>(top);
-        }
-        scales.b[0] = scale_byte(top);
+        top = group_max<V>(top);
     }
+    const unsigned b = scale_byte(top);
+    const Pair inverse(scale_inverse(b));
     auto codes = [&](int j) {
-        const Pair inverse(scale_inverse(scales.b[V == 1 ? j : 0]), scale_inverse(scales.b[V == 1 ? j + 1 : 0]));
         const float2 y = (Pair(x[j], x[j + 1]) * inverse).get();
         return (uint32_t)to_codes(y.x, y.y);
     };
 #pragma unroll
     for (int j = 0; j < N; j += 4) out.w[j / 4] = codes(j) | codes(j + 2) << 16;
+    return b;
 }
 
 // ---- sigmoid --------------------------------------------------------------------------------------------------

@@ -39,8 +39,8 @@ struct Place {
     uint64_t token, wide;  // wide: offset of the lane's values from the token's
     uint64_t code, scale;  // the same in the pool
     uint32_t step, passes;
-    int left, scales_left;  // columns from the unit's first one, and from its groups' first one, on; 0: no unit
-    bool leads, first;
+    int left;          // columns from the unit's first one on; 0: no unit
+    bool leads, first; // leads its group, and so writes the scale; is the token's first unit
     template <typename T>
     __device__ __forceinline__ Place(const Side<T> &s, uint32_t block) {
         const Lane lane(s.tiling, block);
@@ -49,14 +49,13 @@ struct Place {
         passes = s.tiling.passes;
         uint32_t unit;
         const uint32_t head = s.per_row.divmod((uint32_t)lane.unit, unit);
-        const uint32_t column = (uint32_t)Form<V>::column(unit);
+        const uint32_t column = unit * Form<V>::kValues;
         const uint64_t row = (uint64_t)head * s.head_rows;
         wide = head * s.head_stride + column;
         code = row * s.dim + column;
-        scale = row * s.groups + Form<V>::scale(unit);
+        scale = row * s.groups + unit / Form<V>::kLanes;
         left = lane.in && column < s.dim ? (int)(s.dim - column) : 0;
-        scales_left = V == 1 ? left + (int)(column % kGroup) : left;
-        leads = Form<V>::leads(unit);
+        leads = unit % Form<V>::kLanes == 0;
         first = lane.unit == 0;
     }
 };
@@ -88,8 +87,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
     for (int u = 0; u < kPasses; ++u) {
         if (u >= at.passes) break;
         Codes<V> c;
-        Scales<V> b;
-        pack_unit(x[u], c, b);
+        const unsigned b = pack_unit(x[u], c);
         if (slot[u] < 0) continue;
         if ((uint64_t)slot[u] >= pool.slots) {
             if (at.first) raise_error(errors, kErrIndexRange);
@@ -102,7 +100,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
             row += offset;
         }
         c.store(s.codes + row * s.dim + at.code, at.left);
-        if (at.leads) b.store(s.scales + row * s.groups + at.scale, at.scales_left);
+        if (at.leads) s.scales[row * s.groups + at.scale] = (uint8_t)b;
     }
 }
 
@@ -140,7 +138,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
     const int64_t row = first_row + (int64_t)at.token;
     T *to = s.wide + (uint64_t)row * s.token_stride + at.wide;  // not formed into an access before its row is checked
     Codes<V> c[kPasses];
-    Scales<V> scale[kPasses];
+    unsigned scale[kPasses];
     bool live[kPasses];
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
@@ -153,15 +151,16 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
         if (live[u]) {
             const uint64_t from = (uint32_t)page[u] * pool.page_rows + (uint64_t)offset[u] * s.token_rows;
             c[u].load(s.codes + from * s.dim + at.code, at.left);
-            scale[u].load(s.scales + from * s.groups + at.scale, at.scales_left);
+            scale[u] = s.scales[from * s.groups + at.scale];
         }
     }
 #pragma unroll
     for (int u = 0; u < kPasses; ++u) {
         if (!live[u]) continue;
+        const Pair by(scale_value(scale[u]));
         Unit<T, V> y;
 #pragma unroll
-        for (int j = 0; j < Form<V>::kValues; j += 2) y.template set_pair<true>(j, c[u].pair(j, scale[u].pair(j)));
+        for (int j = 0; j < Form<V>::kValues; j += 2) y.template set_pair<true>(j, c[u].pair(j, by));
         y.store(to + u * (at.step * s.token_stride), at.left);
     }
 }

@@ -37,17 +37,17 @@ struct Shape {
 // A lane's column and its rows.
 template <int V>
 struct Place {
-    uint64_t row, column, first_scale;
+    uint64_t row, column, group;
     uint64_t rows_left;  // from `row` on
     uint32_t step, passes;
-    int left;  // columns from the unit's first one on; 0 where it lies behind the row (V > 1: a row ends with a whole unit)
-    bool leads;
+    int left;    // columns from the unit's first one on; 0 where it lies behind the row (V > 1: a row ends with a whole unit)
+    bool leads;  // its group, and so writes the scale
     __device__ __forceinline__ explicit Place(const Shape &s) {
         const Lane lane(s.tiling, blockIdx.x);
         row = lane.line;
-        column = Form<V>::column(lane.unit);
-        first_scale = Form<V>::scale(lane.unit);
-        leads = Form<V>::leads(lane.unit);
+        column = lane.unit * Form<V>::kValues;
+        group = lane.unit / Form<V>::kLanes;
+        leads = lane.unit % Form<V>::kLanes == 0;
         step = s.tiling.side_by_side;
         passes = s.tiling.passes;
         left = lane.in && column < s.cols ? (int)min(s.cols - column, (uint64_t)INT32_MAX) : 0;
@@ -58,10 +58,8 @@ struct Place {
         return p.codes + (row * s.cols + column) + pass * (step * s.cols);
     }
     __device__ __forceinline__ uint8_t *scale(const Packed &p, const Shape &s, int pass) const {
-        return p.scales + (row * s.groups + first_scale) + pass * (step * s.groups);
+        return p.scales + (row * s.groups + group) + pass * (step * s.groups);
     }
-    // columns from the first value of the unit's groups on: what decides which scales there are
-    __device__ __forceinline__ int scales_left(const Shape &s) const { return V == 1 ? left + (int)(column % kGroup) : left; }
     template <typename T>
     __device__ __forceinline__ T *wide(const Rows<T> &r, int pass) const { return r.p + (row * r.stride + column) + pass * (step * r.stride); }
 };
@@ -69,11 +67,10 @@ struct Place {
 template <typename T, int V>
 __device__ __forceinline__ void pack_and_store(const Packed &out, const Shape &s, const Place<V> &at, int pass, const Unit<T, V> &x) {
     Codes<V> c;
-    Scales<V> b;
-    pack_unit(x, c, b);
+    const unsigned b = pack_unit(x, c);
     if (!at.in(pass)) return;
     c.store(at.code(out, s, pass), at.left);
-    if (at.leads) b.store(at.scale(out, s, pass), at.scales_left(s));
+    if (at.leads) *at.scale(out, s, pass) = (uint8_t)b;
 }
 
 template <typename T, int V>
@@ -97,21 +94,22 @@ __global__ void __launch_bounds__(kMaxThreads) unpack_kernel(Rows<T> dst, Packed
     pdl_launch_dependents();
     const Place<V> at(s);
     Codes<V> c[kPassesUnpack];
-    Scales<V> b[kPassesUnpack];
+    unsigned b[kPassesUnpack];
     pdl_wait();
 #pragma unroll
     for (int u = 0; u < kPassesUnpack; ++u) {
         if (u < at.passes && at.in(u)) {
             c[u].load(at.code(in, s, u), at.left);
-            b[u].load(at.scale(in, s, u), at.scales_left(s));
+            b[u] = *at.scale(in, s, u);
         }
     }
 #pragma unroll
     for (int u = 0; u < kPassesUnpack; ++u) {
         if (u >= at.passes || !at.in(u)) continue;
+        const Pair scale(scale_value(b[u]));
         Unit<T, V> y;
 #pragma unroll
-        for (int j = 0; j < Form<V>::kValues; j += 2) y.template set_pair<true>(j, c[u].pair(j, b[u].pair(j)));
+        for (int j = 0; j < Form<V>::kValues; j += 2) y.template set_pair<true>(j, c[u].pair(j, scale));
         y.store(at.wide(dst, u), at.left);
     }
 }
@@ -158,17 +156,14 @@ __global__ void __launch_bounds__(kMaxThreads) silu_mul_grad_kernel(Rows<T> dgat
     if (!at.in(0)) return;
     Unit<T, V> d;
     Codes<V> g, u;
-    Scales<V> gs, us;
-    d.clear();
     d.load(at.wide(dh, 0), at.left);
     g.load(at.code(gate, s, 0), at.left);
     u.load(at.code(up, s, 0), at.left);
-    gs.load(at.scale(gate, s, 0), at.scales_left(s));
-    us.load(at.scale(up, s, 0), at.scales_left(s));
+    const Pair gs(scale_value(*at.scale(gate, s, 0))), us(scale_value(*at.scale(up, s, 0)));
     Unit<T, V> dg, du, y;
 #pragma unroll
     for (int j = 0; j < Form<V>::kValues; j += 2) {
-        const Pair x = g.pair(j, gs.pair(j)), z = u.pair(j, us.pair(j)), dj = d.pair(j);
+        const Pair x = g.pair(j, gs), z = u.pair(j, us), dj = d.pair(j);
         const Sigmoid sg = sigmoid(x);
         const Pair silu = x * sg.s;
         du.template set_pair<false>(j, dj * silu);
