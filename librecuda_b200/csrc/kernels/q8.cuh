@@ -52,14 +52,17 @@ struct FastDiv32 {
 };
 
 // ---- units --------------------------------------------------------------------------------------------------------
-// A unit is kValues consecutive values of a row, held by one lane; kLanes neighbouring lanes hold a group.  Three forms V:
-// 16 values in 32-byte accesses of the wide type, 8 in 16-byte ones, and, as V = 1, 8 values at any address, whose row may
-// end inside the unit.
-template <int V>
+// A unit is kValues consecutive values of a row, held by one lane; kLanes neighbouring lanes hold a group.  Its accesses come
+// in forms A.  32 or 16: bytes of an access to the wide type (the codes then in 16 or 8 bytes).  Rows at any address: in the
+// words that the address allows, 16 values (kLoose) or 8 (kLooseShort).  A loose access of a lane is a word of its own
+// stretch, so a warp touches many sectors at once; loads find them again in L1, stores do not, so kernels that store the
+// wide type at any address use the short form (unpacking 16384x8191 to bf16: 128 us against 244).
+// With A = 32 a row ends with a whole unit, with A = 16 after 8 or 16 of its values, in a loose form anywhere.
+constexpr int kLoose = 4, kLooseShort = 2;
+template <int A>
 struct Form {
-    static constexpr int kValues = V == 1 ? 8 : V;
+    static constexpr int kValues = A == kLooseShort ? 8 : 16;
     static constexpr int kLanes = kGroup / kValues;
-    __host__ __device__ static uint64_t per_row(uint64_t groups) { return groups * kLanes; }
 };
 
 // ---- which units a lane works on --------------------------------------------------------------------------------
@@ -67,15 +70,15 @@ struct Form {
 // CTA takes `passes` units per lane, at the same place of as many lines, so a lane knows its column once and only steps its
 // pointers from line to line.  Lines of up to kMaxThreads units: several lie side by side in a CTA.  Longer ones: `chunks`
 // CTAs share a line in even parts.  Parts start at multiples of 32 lanes, lines at multiples of a group's lanes, so
-// the lanes of a group are neighbours in one warp.  Little work is spread over more CTAs with fewer passes.
+// the lanes of a group are neighbours in one warp.  A grid that would not fill the GPU that way takes one pass.
 constexpr int kMaxThreads = 128;
 struct Tiling {
     uint64_t width, lines;
     FastDiv32 by_chunks, by_width;  // by_width: of lines that lie side by side, else 0 / 1
     uint32_t threads, side_by_side, passes;
     // `times`: how often the launch repeats the tiling
-    static Tiling of(uint64_t lines, uint64_t width, uint32_t max_passes, uint64_t times = 1) {
-        Tiling t{width, lines, FastDiv32::of(1), FastDiv32::of(1), 0, 1, 1};
+    static Tiling of(uint64_t lines, uint64_t width, uint32_t passes, uint64_t times = 1) {
+        Tiling t{width, lines, FastDiv32::of(1), FastDiv32::of(1), 0, 1, passes};
         if (width <= kMaxThreads) {
             t.by_width = FastDiv32::of((uint32_t)width);
             t.side_by_side = (uint32_t)(kMaxThreads / width);
@@ -86,10 +89,10 @@ struct Tiling {
             t.by_chunks = FastDiv32::of((uint32_t)chunks);
             t.threads = (uint32_t)(((width + chunks - 1) / chunks + 31) / 32 * 32);
         }
-        const uint64_t resident = (uint64_t)sm_count() * (2048 / kMaxThreads);
-        while (t.passes < max_passes && lines > (uint64_t)t.side_by_side * t.passes && t.blocks() * times > 2 * resident) t.passes *= 2;
+        if (t.blocks() * times < resident_ctas()) t.passes = 1;
         return t;
     }
+    static uint64_t resident_ctas() { return (uint64_t)sm_count() * (2048 / kMaxThreads); }
     uint64_t blocks() const {
         const uint64_t tile = (uint64_t)side_by_side * passes;
         return (lines + tile - 1) / tile * by_chunks.d;
@@ -99,16 +102,16 @@ struct Lane {
     uint64_t line;  // of the first pass; the next ones are side_by_side further each
     uint64_t unit;  // of the line
     bool in;        // has a unit; lanes without one still take part in a warp's votes and shuffles
-    __device__ __forceinline__ Lane(const Tiling &t, uint32_t block) {
+    __device__ __forceinline__ Lane(const Tiling &t, uint32_t block, uint32_t passes) {
         uint32_t chunk, place;
         const uint32_t tile = t.by_chunks.divmod(block, chunk);
         if (t.by_chunks.d == 1) {
             const uint32_t local = t.by_width.divmod(threadIdx.x, place);
-            line = (uint64_t)tile * (t.side_by_side * t.passes) + local;
+            line = (uint64_t)tile * (t.side_by_side * passes) + local;
             unit = place;
             in = local < t.side_by_side;
         } else {
-            line = (uint64_t)tile * t.passes;
+            line = (uint64_t)tile * passes;
             unit = (uint64_t)chunk * t.threads + threadIdx.x;
             in = unit < t.width && threadIdx.x < t.threads;  // a CTA may be wider than this tiling asks for
         }
@@ -171,10 +174,11 @@ __device__ __forceinline__ uint32_t pair_from_f32(float lo, float hi) {
     return r;
 }
 
-template <typename T, int V>
+template <typename T, int A>
 struct Unit {  // as it lies in memory
-    static constexpr int kValues = Form<V>::kValues;
+    static constexpr int kValues = Form<A>::kValues;
     static constexpr int kWords = kValues * (int)sizeof(T) / 4;
+    static constexpr int kPerWord = 4 / (int)sizeof(T);
     uint32_t w[kWords];
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -182,25 +186,26 @@ struct Unit {  // as it lies in memory
     }
     // `left` > 0: columns from the unit's first one to the end of the row.  Values behind the end are 0.
     __device__ __forceinline__ void load(const T *p, int left) {
-        if constexpr (V == 16) {
+        const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+        if constexpr (A == 32) {
 #pragma unroll
             for (int i = 0; i < kWords; i += 8)
                 asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                              : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
-                             : "l"(reinterpret_cast<const uint32_t *>(p) + i));
-        } else if constexpr (V == 8) {
+                             : "l"(q + i));
+        } else if constexpr (A == 16) {  // the lanes' accesses interleave: the second one finds its sectors in L1
 #pragma unroll
             for (int i = 0; i < kWords; i += 4) {
-                const uint4 v = ld_stream<2>(reinterpret_cast<const uint4 *>(p) + i / 4);
+                const uint4 v = i * kPerWord < left ? ld_stream<1>(reinterpret_cast<const uint4 *>(q + i)) : make_uint4(0, 0, 0, 0);
                 w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
             }
         } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) w[i] = i < left ? reinterpret_cast<const uint32_t *>(p)[i] : 0u;
+            for (int i = 0; i < kWords; ++i) w[i] = i < left ? q[i] : 0u;
         } else {
             // the aligned words that hold at least one of the values, shifted by half a word where the address asks for it
             const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(p) >> 1) & 1u;
-            const uint32_t *q = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+            q = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
             const int n = min(left, kValues) + (int)odd;
             uint32_t r[kWords + 1];
 #pragma unroll
@@ -214,20 +219,21 @@ struct Unit {  // as it lies in memory
         }
     }
     __device__ __forceinline__ void store(T *p, int left) const {
-        if constexpr (V == 16) {
+        uint32_t *q = reinterpret_cast<uint32_t *>(p);
+        if constexpr (A == 32) {
 #pragma unroll
             for (int i = 0; i < kWords; i += 8)
                 asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                             :: "l"(reinterpret_cast<uint32_t *>(p) + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
-                                "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7]) : "memory");
-        } else if constexpr (V == 8) {
+                             :: "l"(q + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                             : "memory");
+        } else if constexpr (A == 16) {
 #pragma unroll
             for (int i = 0; i < kWords; i += 4)
-                st_stream<2>(reinterpret_cast<uint4 *>(p) + i / 4, make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+                if (i * kPerWord < left) st_stream<1>(reinterpret_cast<uint4 *>(q + i), make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
         } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < kWords; ++i)
-                if (i < left) reinterpret_cast<uint32_t *>(p)[i] = w[i];
+                if (i < left) q[i] = w[i];
         } else {
             uint16_t *h = reinterpret_cast<uint16_t *>(p);
             if (left < kValues) {
@@ -236,7 +242,7 @@ struct Unit {  // as it lies in memory
                     if (j < left) h[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
             } else if ((reinterpret_cast<uintptr_t>(p) & 2) == 0) {
 #pragma unroll
-                for (int i = 0; i < kWords; ++i) reinterpret_cast<uint32_t *>(p)[i] = w[i];
+                for (int i = 0; i < kWords; ++i) q[i] = w[i];
             } else {
                 h[0] = (uint16_t)w[0];
 #pragma unroll
@@ -299,10 +305,10 @@ __device__ __forceinline__ float nan_if_infinite(float x) {
 }
 
 // Largest over the lanes of a group; every lane of the warp calls it.
-template <int V>
+template <int A>
 __device__ __forceinline__ unsigned group_max(unsigned m) {
 #pragma unroll
-    for (int o = 1; o < Form<V>::kLanes; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = 1; o < Form<A>::kLanes; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     return m;
 }
 
@@ -312,55 +318,59 @@ __device__ __forceinline__ uint16_t to_codes(float lo, float hi) {  // saturates
     return r;
 }
 
-template <int V>
+template <int A>
 struct Codes {  // of one unit, four to a word
-    static constexpr int kValues = Form<V>::kValues;
-    uint32_t w[kValues / 4];
+    static constexpr int kValues = Form<A>::kValues;
+    static constexpr int kWords = kValues / 4;
+    uint32_t w[kWords];
     __device__ __forceinline__ void load(const uint8_t *p, int left) {
-        if constexpr (V == 16) {
+        if constexpr (A == 32) {
             const uint4 v = ld_stream<2>(reinterpret_cast<const uint4 *>(p));
             w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-        } else if constexpr (V == 8) {
-            asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+        } else if constexpr (A == 16) {
+            const uint2 *q = reinterpret_cast<const uint2 *>(p);
+            const uint2 lo = q[0], hi = left > 8 ? q[1] : make_uint2(0, 0);
+            w[0] = lo.x, w[1] = lo.y, w[2] = hi.x, w[3] = hi.y;
         } else {
             // the aligned words that hold at least one of the codes; codes behind the row's end are whatever lies there
             const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3);
             const uint32_t *q = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
             const int n = min(left, kValues) + (int)shift;
-            uint32_t r[3];
+            uint32_t r[kWords + 1];
 #pragma unroll
-            for (int i = 0; i < 3; ++i) r[i] = 4 * i < n ? q[i] : 0u;
-            w[0] = __funnelshift_r(r[0], r[1], 8 * shift);
-            w[1] = __funnelshift_r(r[1], r[2], 8 * shift);
+            for (int i = 0; i <= kWords; ++i) r[i] = 4 * i < n ? q[i] : 0u;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(r[i], r[i + 1], 8 * shift);
         }
     }
     __device__ __forceinline__ void store(uint8_t *p, int left) const {
-        if constexpr (V == 16) st_stream<2>(reinterpret_cast<uint4 *>(p), make_uint4(w[0], w[1], w[2], w[3]));
-        else if constexpr (V == 8) asm volatile("st.global.L1::no_allocate.v2.u32 [%0], {%1,%2};" :: "l"(p), "r"(w[0]), "r"(w[1]) : "memory");
-        else if (left < kValues) {
+        if constexpr (A == 32) st_stream<2>(reinterpret_cast<uint4 *>(p), make_uint4(w[0], w[1], w[2], w[3]));
+        else if constexpr (A == 16) {
+            uint2 *q = reinterpret_cast<uint2 *>(p);
+            q[0] = make_uint2(w[0], w[1]);
+            if (left > 8) q[1] = make_uint2(w[2], w[3]);
+        } else if (left < kValues) {
 #pragma unroll
             for (int j = 0; j < kValues; ++j)
                 if (j < left) p[j] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
         } else {
-            // the widest accesses that the address allows: 1, 2 and 4 bytes in some order
             const uint32_t m = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3);
             if (m == 0) {
-                reinterpret_cast<uint32_t *>(p)[0] = w[0];
-                reinterpret_cast<uint32_t *>(p)[1] = w[1];
-            } else if (m == 2) {
-                *reinterpret_cast<uint16_t *>(p) = (uint16_t)w[0];
-                *reinterpret_cast<uint32_t *>(p + 2) = __funnelshift_r(w[0], w[1], 16);
-                *reinterpret_cast<uint16_t *>(p + 6) = (uint16_t)(w[1] >> 16);
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) reinterpret_cast<uint32_t *>(p)[i] = w[i];
             } else {
-                p[0] = (uint8_t)w[0];
-                if (m == 1) {
-                    *reinterpret_cast<uint16_t *>(p + 1) = (uint16_t)(w[0] >> 8);
-                    *reinterpret_cast<uint32_t *>(p + 3) = __funnelshift_r(w[0], w[1], 24);
-                } else {
-                    *reinterpret_cast<uint32_t *>(p + 1) = __funnelshift_r(w[0], w[1], 8);
-                    *reinterpret_cast<uint16_t *>(p + 5) = (uint16_t)(w[1] >> 8);
-                }
-                p[7] = (uint8_t)(w[1] >> 24);
+                // up to the first word's boundary, the words between, and what is left of the last word
+                if (m == 2) *reinterpret_cast<uint16_t *>(p) = (uint16_t)w[0];
+                else p[0] = (uint8_t)w[0];
+                if (m == 1) *reinterpret_cast<uint16_t *>(p + 1) = (uint16_t)(w[0] >> 8);
+                uint32_t *q = reinterpret_cast<uint32_t *>(p + (4 - m));
+#pragma unroll
+                for (int i = 0; i + 1 < kWords; ++i) q[i] = __funnelshift_r(w[i], w[i + 1], 8 * (4 - m));
+                const uint32_t rest = w[kWords - 1] >> (8 * (4 - m));
+                uint8_t *e = reinterpret_cast<uint8_t *>(q + kWords - 1);
+                if (m != 1) *reinterpret_cast<uint16_t *>(e) = (uint16_t)rest;
+                if (m == 1) e[0] = (uint8_t)rest;
+                if (m == 3) e[2] = (uint8_t)(rest >> 16);
             }
         }
     }
@@ -376,13 +386,13 @@ struct Codes {  // of one unit, four to a word
 // Packs a unit; returns the scale byte of its group.  Every lane of the warp calls it; lanes without values come with a
 // cleared unit.  The maximum ignores NaN, which convert to the NaN code by themselves; infinities are rare, so only when one
 // is found somewhere in the warp the values are looked at one by one.
-template <typename T, int V>
-__device__ __forceinline__ unsigned pack_unit(const Unit<T, V> &in, Codes<V> &out) {
-    constexpr int N = Form<V>::kValues;
+template <typename T, int A>
+__device__ __forceinline__ unsigned pack_unit(const Unit<T, A> &in, Codes<A> &out) {
+    constexpr int N = Form<A>::kValues;
     float x[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = in.value(j);
-    unsigned top = group_max<V>(in.top_bits());
+    unsigned top = group_max<A>(in.top_bits());
     if (__any_sync(0xffffffffu, top >= kInfBits)) {
         top = 0;
 #pragma unroll
@@ -390,7 +400,7 @@ __device__ __forceinline__ unsigned pack_unit(const Unit<T, V> &in, Codes<V> &ou
             top = max(top, finite_magnitude(x[j]));
             x[j] = nan_if_infinite(x[j]);
         }
-        top = group_max<V>(top);
+        top = group_max<A>(top);
     }
     const unsigned b = scale_byte(top);
     const Pair inverse(scale_inverse(b));
@@ -440,14 +450,20 @@ int with_type(int type, Fn fn) {
     }
 }
 
-// calls fn with std::integral_constant of the unit
-template <typename Fn>
-int with_unit(int v, Fn fn) {
-    switch (v) {
+// calls fn with std::integral_constant of the access form; 0: the loose one
+template <int LOOSE, typename Fn>
+int with_access(int a, Fn fn) {
+    switch (a) {
+        case 32: return fn(std::integral_constant<int, 32>());
         case 16: return fn(std::integral_constant<int, 16>());
-        case 8: return fn(std::integral_constant<int, 8>());
-        default: return fn(std::integral_constant<int, 1>());
+        default: return fn(std::integral_constant<int, LOOSE>());
     }
+}
+
+// calls fn with std::integral_constant of the passes: 1 or MOST
+template <int MOST, typename Fn>
+int with_passes(uint32_t passes, Fn fn) {
+    return passes == 1 ? fn(std::integral_constant<int, 1>()) : fn(std::integral_constant<int, MOST>());
 }
 
 // ---- an index out of range in device memory -----------------------------------------------------------------------

@@ -9,8 +9,9 @@
 namespace lcb {
 namespace {
 
-// units in flight per lane, at most
-constexpr int kPasses = 4;
+// Units in flight per lane, where there is work for that many.
+template <int A>
+constexpr int kPassesPack = A >= 16 ? 4 : 2;
 constexpr int kPassesUnpack = 2;
 constexpr int kPassesSilu = 2;  // of each input
 constexpr int kPassesGrad = 1;
@@ -24,145 +25,157 @@ struct Packed {
     uint8_t *codes, *scales;
 };
 
+// A matrix whose rows lie behind each other without a gap and end with whole groups is one long row, and so is a single row.  It
+// is cut into lines of kMaxThreads units, which keeps every lane busy whatever the number of columns.
 struct Shape {
     uint64_t rows, cols, groups;
+    uint64_t flat;  // values of one long row, else 0
     Tiling tiling;
-    template <int V>
-    static Shape of(size_t rows, size_t cols, int max_passes) {
+    template <int A>
+    static Shape of(size_t rows, size_t cols, bool flat, int passes) {
+        if (flat) {
+            const uint64_t line = kMaxThreads * Form<A>::kValues, total = (uint64_t)rows * cols, lines = (total + line - 1) / line;
+            return {lines, line, line / kGroup, total, Tiling::of(lines, kMaxThreads, passes)};
+        }
         const uint64_t groups = groups_of(cols);
-        return {rows, cols, groups, Tiling::of(rows, Form<V>::per_row(groups), max_passes)};
+        return {rows, cols, groups, 0, Tiling::of(rows, groups * Form<A>::kLanes, passes)};
     }
 };
 
-// A lane's column and its rows.
-template <int V>
+// A lane's column and its rows, P passes of them.
+template <int A, int P>
 struct Place {
-    uint64_t row, column, group;
-    uint64_t rows_left;  // from `row` on
-    uint32_t step, passes;
-    int left;    // columns from the unit's first one on; 0 where it lies behind the row (V > 1: a row ends with a whole unit)
-    bool leads;  // its group, and so writes the scale
+    uint64_t row, column;
+    uint64_t code, scale;  // of the unit in the packed matrix
+    uint32_t step;         // rows from pass to pass
+    uint32_t live;         // passes in which this lane has a unit: the first ones
+    int left, last;        // columns from the unit's first one on, and in the last live pass
+    bool leads;            // its group, and so writes the scale
     __device__ __forceinline__ explicit Place(const Shape &s) {
-        const Lane lane(s.tiling, blockIdx.x);
+        const Lane lane(s.tiling, blockIdx.x, P);
         row = lane.line;
-        column = lane.unit * Form<V>::kValues;
-        group = lane.unit / Form<V>::kLanes;
-        leads = lane.unit % Form<V>::kLanes == 0;
+        column = lane.unit * Form<A>::kValues;
+        code = row * s.cols + column;
+        scale = row * s.groups + lane.unit / Form<A>::kLanes;
+        leads = lane.unit % Form<A>::kLanes == 0;
         step = s.tiling.side_by_side;
-        passes = s.tiling.passes;
-        left = lane.in && column < s.cols ? (int)min(s.cols - column, (uint64_t)INT32_MAX) : 0;
-        rows_left = row < s.rows ? s.rows - row : 0;
+        const uint64_t end = s.flat != 0 ? s.flat : s.rows, at = s.flat != 0 ? code : row;
+        const uint32_t rest = lane.in && column < s.cols && at < end ? (uint32_t)min(end - at, (uint64_t)INT32_MAX) : 0;
+        const uint32_t stride = s.flat != 0 ? step * (uint32_t)s.cols : step;
+        live = 0;
+#pragma unroll
+        for (uint32_t u = 0; u < P; ++u) live += u * stride < rest;
+        left = last = (int)min(s.cols - column, (uint64_t)INT32_MAX);
+        if (s.flat != 0 && live != 0) last = min(left, (int)(rest - (live - 1) * stride));
     }
-    __device__ __forceinline__ bool in(int pass) const { return left > 0 && pass * step < rows_left; }
-    __device__ __forceinline__ uint8_t *code(const Packed &p, const Shape &s, int pass) const {
-        return p.codes + (row * s.cols + column) + pass * (step * s.cols);
-    }
-    __device__ __forceinline__ uint8_t *scale(const Packed &p, const Shape &s, int pass) const {
-        return p.scales + (row * s.groups + group) + pass * (step * s.groups);
-    }
+    __device__ __forceinline__ int columns(uint32_t pass) const { return pass + 1 == live ? last : left; }
     template <typename T>
-    __device__ __forceinline__ T *wide(const Rows<T> &r, int pass) const { return r.p + (row * r.stride + column) + pass * (step * r.stride); }
+    __device__ __forceinline__ T *wide(const Rows<T> &r) const { return r.p + (row * r.stride + column); }
 };
 
-template <typename T, int V>
-__device__ __forceinline__ void pack_and_store(const Packed &out, const Shape &s, const Place<V> &at, int pass, const Unit<T, V> &x) {
-    Codes<V> c;
+template <typename T, int A, int P>
+__device__ __forceinline__ void pack_and_store(const Packed &out, const Shape &s, const Place<A, P> &at, uint32_t pass, const Unit<T, A> &x) {
+    Codes<A> c;
     const unsigned b = pack_unit(x, c);
-    if (!at.in(pass)) return;
-    c.store(at.code(out, s, pass), at.left);
-    if (at.leads) *at.scale(out, s, pass) = (uint8_t)b;
+    if (pass >= at.live) return;
+    c.store(out.codes + at.code + pass * (at.step * s.cols), at.columns(pass));
+    if (at.leads) out.scales[at.scale + pass * (at.step * s.groups)] = (uint8_t)b;
 }
 
-template <typename T, int V>
+template <typename T, int A, int P>
 __global__ void __launch_bounds__(kMaxThreads) pack_kernel(Packed out, Rows<const T> src, Shape s) {
     pdl_launch_dependents();
-    const Place<V> at(s);
-    Unit<T, V> x[kPasses];
+    const Place<A, P> at(s);
+    const T *from = at.wide(src);
+    Unit<T, A> x[P];
     pdl_wait();
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
+    for (uint32_t u = 0; u < P; ++u) {
         x[u].clear();
-        if (u < at.passes && at.in(u)) x[u].load(at.wide(src, u), at.left);
+        if (u < at.live) x[u].load(from + u * (at.step * src.stride), at.columns(u));
     }
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u)
-        if (u < at.passes) pack_and_store(out, s, at, u, x[u]);
+    for (uint32_t u = 0; u < P; ++u)
+        pack_and_store(out, s, at, u, x[u]);
 }
 
-template <typename T, int V>
+template <typename T, int A, int P>
 __global__ void __launch_bounds__(kMaxThreads) unpack_kernel(Rows<T> dst, Packed in, Shape s) {
     pdl_launch_dependents();
-    const Place<V> at(s);
-    Codes<V> c[kPassesUnpack];
-    unsigned b[kPassesUnpack];
+    const Place<A, P> at(s);
+    T *to = at.wide(dst);
+    const uint8_t *codes = in.codes + at.code, *scales = in.scales + at.scale;
+    Codes<A> c[P];
+    unsigned b[P];
     pdl_wait();
 #pragma unroll
-    for (int u = 0; u < kPassesUnpack; ++u) {
-        if (u < at.passes && at.in(u)) {
-            c[u].load(at.code(in, s, u), at.left);
-            b[u] = *at.scale(in, s, u);
+    for (uint32_t u = 0; u < P; ++u) {
+        if (u < at.live) {
+            c[u].load(codes + u * (at.step * s.cols), at.columns(u));
+            b[u] = scales[u * (at.step * s.groups)];
         }
     }
 #pragma unroll
-    for (int u = 0; u < kPassesUnpack; ++u) {
-        if (u >= at.passes || !at.in(u)) continue;
+    for (uint32_t u = 0; u < P; ++u) {
+        if (u >= at.live) break;
         const Pair scale(scale_value(b[u]));
-        Unit<T, V> y;
+        Unit<T, A> y;
 #pragma unroll
-        for (int j = 0; j < Form<V>::kValues; j += 2) y.template set_pair<true>(j, c[u].pair(j, scale));
-        y.store(at.wide(dst, u), at.left);
+        for (int j = 0; j < Form<A>::kValues; j += 2) y.template set_pair<true>(j, c[u].pair(j, scale));
+        y.store(to + u * (at.step * dst.stride), at.columns(u));
     }
 }
 
-template <typename T, int V>
+template <typename T, int A, int P>
 __global__ void __launch_bounds__(kMaxThreads) silu_mul_pack_kernel(Rows<T> h, Packed gate_out, Packed up_out, Rows<const T> gate,
                                                                     Rows<const T> up, Shape s) {
     pdl_launch_dependents();
-    const Place<V> at(s);
-    Unit<T, V> g[kPassesSilu], u[kPassesSilu];
+    const Place<A, P> at(s);
+    const T *from_gate = at.wide(gate), *from_up = at.wide(up);
+    T *to = at.wide(h);
+    Unit<T, A> g[P], u[P];
     pdl_wait();
 #pragma unroll
-    for (int k = 0; k < kPassesSilu; ++k) {
+    for (uint32_t k = 0; k < P; ++k) {
         g[k].clear();
         u[k].clear();
-        if (k < at.passes && at.in(k)) {
-            g[k].load(at.wide(gate, k), at.left);
-            u[k].load(at.wide(up, k), at.left);
+        if (k < at.live) {
+            g[k].load(from_gate + k * (at.step * gate.stride), at.columns(k));
+            u[k].load(from_up + k * (at.step * up.stride), at.columns(k));
         }
     }
 #pragma unroll
-    for (int k = 0; k < kPassesSilu; ++k) {
-        if (k >= at.passes) break;
-        if (at.in(k)) {
-            Unit<T, V> out;
+    for (uint32_t k = 0; k < P; ++k) {
+        if (k < at.live) {
+            Unit<T, A> out;
 #pragma unroll
-            for (int j = 0; j < Form<V>::kValues; j += 2) {
+            for (int j = 0; j < Form<A>::kValues; j += 2) {
                 const Pair x = g[k].pair(j);
                 out.template set_pair<false>(j, x * sigmoid(x).s * u[k].pair(j));
             }
-            out.store(at.wide(h, k), at.left);
+            out.store(to + k * (at.step * h.stride), at.columns(k));
         }
         pack_and_store(gate_out, s, at, k, g[k]);
         pack_and_store(up_out, s, at, k, u[k]);
     }
 }
 
-template <typename T, int V, bool AGAIN>
+template <typename T, int A, bool AGAIN>
 __global__ void __launch_bounds__(kMaxThreads) silu_mul_grad_kernel(Rows<T> dgate, Rows<T> dup, Rows<T> h, Rows<const T> dh, Packed gate,
                                                                     Packed up, Shape s) {
     pdl_launch_dependents();
-    const Place<V> at(s);
+    const Place<A, 1> at(s);
     pdl_wait();
-    if (!at.in(0)) return;
-    Unit<T, V> d;
-    Codes<V> g, u;
-    d.load(at.wide(dh, 0), at.left);
-    g.load(at.code(gate, s, 0), at.left);
-    u.load(at.code(up, s, 0), at.left);
-    const Pair gs(scale_value(*at.scale(gate, s, 0))), us(scale_value(*at.scale(up, s, 0)));
-    Unit<T, V> dg, du, y;
+    if (at.live == 0) return;
+    Unit<T, A> d;
+    Codes<A> g, u;
+    d.load(at.wide(dh), at.last);
+    g.load(gate.codes + at.code, at.last);
+    u.load(up.codes + at.code, at.last);
+    const Pair gs(scale_value(gate.scales[at.scale])), us(scale_value(up.scales[at.scale]));
+    Unit<T, A> dg, du, y;
 #pragma unroll
-    for (int j = 0; j < Form<V>::kValues; j += 2) {
+    for (int j = 0; j < Form<A>::kValues; j += 2) {
         const Pair x = g.pair(j, gs), z = u.pair(j, us), dj = d.pair(j);
         const Sigmoid sg = sigmoid(x);
         const Pair silu = x * sg.s;
@@ -170,27 +183,44 @@ __global__ void __launch_bounds__(kMaxThreads) silu_mul_grad_kernel(Rows<T> dgat
         dg.template set_pair<false>(j, dj * z * fma2(silu, sg.q, sg.s));
         if constexpr (AGAIN) y.template set_pair<false>(j, silu * z);
     }
-    du.store(at.wide(dup, 0), at.left);
-    dg.store(at.wide(dgate, 0), at.left);
-    if constexpr (AGAIN) y.store(at.wide(h, 0), at.left);
+    du.store(at.wide(dup), at.last);
+    dg.store(at.wide(dgate), at.last);
+    if constexpr (AGAIN) y.store(at.wide(h), at.last);
 }
 
-// The widest unit whose accesses are aligned in every row: codes and values of a unit start at multiples of its size.
-// A row's codes lie behind each other, so the columns must be a multiple of the unit; 16 values take 32-byte accesses of the
-// wide type (f32: two) and 16-byte ones of the codes, 8 values half of that.
+// The widest accesses that are aligned in every row.  A row's codes lie behind each other, so the columns must be a multiple of
+// what an access covers.
 struct Fit {
+    size_t rows, cols;
+    bool flat;
     uint64_t wide = 0, codes = 0;
+    Fit(size_t rows, size_t cols) : rows(rows), cols(cols), flat(rows == 1 || cols % kGroup == 0) {}
     template <typename T>
-    void add(const Rows<T> &r, size_t rows) {
-        if (r.p != nullptr) wide |= reinterpret_cast<uintptr_t>(r.p) | (rows > 1 ? r.stride * sizeof(T) : 0);
+    void add(const Rows<T> &r) {
+        if (r.p == nullptr) return;
+        wide |= reinterpret_cast<uintptr_t>(r.p) | (rows > 1 ? r.stride * sizeof(T) : 0);
+        if (rows > 1 && r.stride != cols) flat = false;
     }
     void add(const Packed &p) { codes |= reinterpret_cast<uintptr_t>(p.codes); }
-    int unit(size_t cols) const {
-        if (cols % 16 == 0 && wide % 32 == 0 && codes % 16 == 0) return 16;
-        if (cols % 8 == 0 && wide % 16 == 0 && codes % 8 == 0) return 8;
-        return 1;
+    int access() const {
+        if (cols % 16 == 0 && wide % 32 == 0 && codes % 16 == 0) return 32;
+        if (cols % 8 == 0 && wide % 16 == 0 && codes % 8 == 0) return 16;
+        return 0;
     }
+    // one long row is addressed in lines that lie behind each other
+    template <typename T>
+    Rows<T> lines(const Rows<T> &r, const Shape &s) const { return {r.p, flat ? (size_t)s.cols : r.stride}; }
 };
+
+// A single row whose number of columns is no multiple of a group is done in two parts, so that the last group does not
+// decide how all the others are read.  part(first column, columns)
+template <typename Part>
+int in_parts(size_t rows, size_t cols, Part part) {
+    const size_t body = cols / kGroup * kGroup;
+    if (rows != 1 || body == cols || body == 0) return part(0, cols);
+    const int rc = part(0, body);
+    return rc != 0 ? rc : part(body, cols - body);
+}
 
 template <typename... KArgs, typename... Args>
 int launch_rows(void (*kernel)(KArgs...), const Shape &s, lcbStream stream, Args... args) {
@@ -202,8 +232,9 @@ int launch_rows(void (*kernel)(KArgs...), const Shape &s, lcbStream stream, Args
 Packed packed(const void *codes, const void *scales) {
     return {static_cast<uint8_t *>(const_cast<void *>(codes)), static_cast<uint8_t *>(const_cast<void *>(scales))};
 }
+Packed from(const Packed &p, size_t column) { return {p.codes + column, p.scales + column / kGroup}; }
 template <typename T, typename P>
-Rows<T> rows_at(P *p, size_t stride) { return {static_cast<T *>(p), stride}; }
+Rows<T> rows_at(P *p, size_t stride, size_t column) { return {p != nullptr ? static_cast<T *>(p) + column : nullptr, stride}; }
 
 }  // namespace
 }  // namespace lcb
@@ -216,13 +247,18 @@ extern "C" int lcb_pack_q8(void *codes, void *scales, const void *src, size_t sr
     if (rows == 0 || cols == 0) return 0;
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const auto in = rows_at<const T>(src, src_stride);
-        const Packed out = packed(codes, scales);
-        Fit fit;
-        fit.add(in, rows);
-        fit.add(out);
-        return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(pack_kernel<T, v()>, Shape::of<v()>(rows, cols, kPasses), stream, out, in);
+        return in_parts(rows, cols, [&](size_t column, size_t n) {
+            const auto in = rows_at<const T>(src, src_stride, column);
+            const Packed out = from(packed(codes, scales), column);
+            Fit fit(rows, n);
+            fit.add(in);
+            fit.add(out);
+            return with_access<kLoose>(fit.access(), [&](auto a) {
+                const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesPack<a()>);
+                return with_passes<kPassesPack<a()>>(s.tiling.passes, [&](auto p) {
+                    return launch_rows(pack_kernel<T, a(), p()>, s, stream, out, fit.lines(in, s));
+                });
+            });
         });
     });
 }
@@ -233,13 +269,18 @@ extern "C" int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void 
     if (rows == 0 || cols == 0) return 0;
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const auto out = rows_at<T>(dst, dst_stride);
-        const Packed in = packed(codes, scales);
-        Fit fit;
-        fit.add(out, rows);
-        fit.add(in);
-        return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(unpack_kernel<T, v()>, Shape::of<v()>(rows, cols, kPassesUnpack), stream, out, in);
+        return in_parts(rows, cols, [&](size_t column, size_t n) {
+            const auto out = rows_at<T>(dst, dst_stride, column);
+            const Packed in = from(packed(codes, scales), column);
+            Fit fit(rows, n);
+            fit.add(out);
+            fit.add(in);
+            return with_access<kLooseShort>(fit.access(), [&](auto a) {
+                const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesUnpack);
+                return with_passes<kPassesUnpack>(s.tiling.passes, [&](auto p) {
+                    return launch_rows(unpack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), in);
+                });
+            });
         });
     });
 }
@@ -251,17 +292,22 @@ extern "C" int lcb_silu_mul_pack_q8(void *h, size_t h_stride, void *gate_codes, 
     if (rows == 0 || cols == 0) return 0;
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const auto out = rows_at<T>(h, h_stride);
-        const auto g = rows_at<const T>(gate, gate_stride), u = rows_at<const T>(up, up_stride);
-        const Packed gp = packed(gate_codes, gate_scales), upk = packed(up_codes, up_scales);
-        Fit fit;
-        fit.add(out, rows);
-        fit.add(g, rows);
-        fit.add(u, rows);
-        fit.add(gp);
-        fit.add(upk);
-        return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(silu_mul_pack_kernel<T, v()>, Shape::of<v()>(rows, cols, kPassesSilu), stream, out, gp, upk, g, u);
+        return in_parts(rows, cols, [&](size_t column, size_t n) {
+            const auto out = rows_at<T>(h, h_stride, column);
+            const auto g = rows_at<const T>(gate, gate_stride, column), u = rows_at<const T>(up, up_stride, column);
+            const Packed gp = from(packed(gate_codes, gate_scales), column), upk = from(packed(up_codes, up_scales), column);
+            Fit fit(rows, n);
+            fit.add(out);
+            fit.add(g);
+            fit.add(u);
+            fit.add(gp);
+            fit.add(upk);
+            return with_access<kLooseShort>(fit.access(), [&](auto a) {
+                const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesSilu);
+                return with_passes<kPassesSilu>(s.tiling.passes, [&](auto p) {
+                    return launch_rows(silu_mul_pack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), gp, upk, fit.lines(g, s), fit.lines(u, s));
+                });
+            });
         });
     });
 }
@@ -275,19 +321,22 @@ extern "C" int lcb_silu_mul_grad_q8(void *dgate, size_t dgate_stride, void *dup,
     if (rows == 0 || cols == 0) return 0;
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const auto dg = rows_at<T>(dgate, dgate_stride), du = rows_at<T>(dup, dup_stride), out = rows_at<T>(h, h_stride);
-        const auto d = rows_at<const T>(dh, dh_stride);
-        const Packed gp = packed(gate_codes, gate_scales), upk = packed(up_codes, up_scales);
-        Fit fit;
-        fit.add(dg, rows);
-        fit.add(du, rows);
-        fit.add(out, rows);
-        fit.add(d, rows);
-        fit.add(gp);
-        fit.add(upk);
-        return with_unit(fit.unit(cols), [&](auto v) {
-            return launch_rows(h != nullptr ? silu_mul_grad_kernel<T, v(), true> : silu_mul_grad_kernel<T, v(), false>,
-                               Shape::of<v()>(rows, cols, kPassesGrad), stream, dg, du, out, d, gp, upk);
+        return in_parts(rows, cols, [&](size_t column, size_t n) {
+            const auto dg = rows_at<T>(dgate, dgate_stride, column), du = rows_at<T>(dup, dup_stride, column), out = rows_at<T>(h, h_stride, column);
+            const auto d = rows_at<const T>(dh, dh_stride, column);
+            const Packed gp = from(packed(gate_codes, gate_scales), column), upk = from(packed(up_codes, up_scales), column);
+            Fit fit(rows, n);
+            fit.add(dg);
+            fit.add(du);
+            fit.add(out);
+            fit.add(d);
+            fit.add(gp);
+            fit.add(upk);
+            return with_access<kLooseShort>(fit.access(), [&](auto a) {
+                const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesGrad);
+                return launch_rows(h != nullptr ? silu_mul_grad_kernel<T, a(), true> : silu_mul_grad_kernel<T, a(), false>, s, stream,
+                                   fit.lines(dg, s), fit.lines(du, s), fit.lines(out, s), fit.lines(d, s), gp, upk);
+            });
         });
     });
 }
