@@ -24,6 +24,7 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "lcb200_types.h"
 #include "librecuda_status.h"
 
 #define LIBRECUDA_EXPORT extern "C"
@@ -180,6 +181,27 @@ LIBRECUDA_EXPORT libreCudaStatus_t libreCuMemsetD16(void *dstDevice, unsigned sh
 LIBRECUDA_EXPORT libreCudaStatus_t libreCuMemsetD16Async(void *dstDevice, unsigned short value, size_t count, LibreCUstream stream);
 LIBRECUDA_EXPORT libreCudaStatus_t libreCuMemsetD32(void *dstDevice, unsigned int value, size_t count, LibreCUstream stream);
 LIBRECUDA_EXPORT libreCudaStatus_t libreCuMemsetD32Async(void *dstDevice, unsigned int value, size_t count, LibreCUstream stream);
+
+// --- 8-bit rows: copies that change the number format ---
+// The kernel layer's 8-bit operators as stream operations; the format (e4m3 codes, one power-of-two scale byte per group of
+// 32 values), the meaning of every argument and what may overlap are described with lcb_pack_q8, lcb_cache_write_q8 and so
+// on in lcb200_kernels.h.  `type` is an enum lcbType, strides are in elements.  All pointers are device memory that the
+// stream's context may access; arguments that the kernel layer refuses, and host pointers, give INVALID_VALUE when the call is
+// recorded.  An lcbCacheQ8 is read when the call is recorded; slots, page tables, lengths and first rows are device memory that
+// is read when the operation runs, so it may be written by work recorded before.  Indices out of range in them are
+// skipped, and the next libreCuStreamAwait on that GPU returns LIBRECUDA_ERROR_UNKNOWN once.
+//
+// Activations in 8 bits: a matrix packed, and read back.  A packed matrix is moved like any other bytes, for instance to
+// pinned host memory and back by libreCuMemCpy on the same stream.
+LIBRECUDA_EXPORT libreCudaStatus_t libreCuPackQ8(void *codes, void *scales, const void *src, size_t srcStride, int type, size_t rows, size_t cols, LibreCUstream stream, bool async = false);
+LIBRECUDA_EXPORT libreCudaStatus_t libreCuUnpackQ8(void *dst, size_t dstStride, int type, const void *codes, const void *scales, size_t rows, size_t cols, LibreCUstream stream, bool async = false);
+// h = gate * up / (1 + exp(-gate)) with gate and up packed in the same pass, and its gradients from the packed pair (h again,
+// unless NULL).
+LIBRECUDA_EXPORT libreCudaStatus_t libreCuSiluMulPackQ8(void *h, size_t hStride, void *gateCodes, void *gateScales, void *upCodes, void *upScales, const void *gate, size_t gateStride, const void *up, size_t upStride, int type, size_t rows, size_t cols, LibreCUstream stream, bool async = false);
+LIBRECUDA_EXPORT libreCudaStatus_t libreCuSiluMulGradQ8(void *dGate, size_t dGateStride, void *dUp, size_t dUpStride, void *h, size_t hStride, const void *dH, size_t dHStride, const void *gateCodes, const void *gateScales, const void *upCodes, const void *upScales, int type, size_t rows, size_t cols, LibreCUstream stream, bool async = false);
+// A paged key/value cache in 8 bits: rows quantised into their slots, and sequences read back through a page table.
+LIBRECUDA_EXPORT libreCudaStatus_t libreCuCacheWriteQ8(const lcbCacheQ8 *cache, const void *k, size_t kTokenStride, size_t kHeadStride, const void *v, size_t vTokenStride, size_t vHeadStride, int type, const int64_t *slots, size_t tokens, LibreCUstream stream, bool async = false);
+LIBRECUDA_EXPORT libreCudaStatus_t libreCuCacheReadQ8(const lcbCacheQ8 *cache, void *k, size_t kTokenStride, size_t kHeadStride, void *v, size_t vTokenStride, size_t vHeadStride, int type, const int32_t *pageTable, size_t tableStride, const int32_t *lengths, const int64_t *firstRows, size_t sequences, size_t maxLength, size_t rows, LibreCUstream stream, bool async = false);
 
 // Make work recorded on `stream` after this call wait, on the GPU, for `event` (recorded on any
 // stream of any context).  The event's stream must be commenced before or together with `stream`;

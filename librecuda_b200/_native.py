@@ -128,6 +128,12 @@ LIBRECU_FUNCTIONS = {
     "libreCuMemsetD16Async": (i32, [vp, C.c_ushort, sz, vp]),
     "libreCuMemsetD32": (i32, [vp, C.c_uint, sz, vp]),
     "libreCuMemsetD32Async": (i32, [vp, C.c_uint, sz, vp]),
+    "libreCuPackQ8": (i32, [vp, vp, vp, sz, i32, sz, sz, vp, C.c_bool]),
+    "libreCuUnpackQ8": (i32, [vp, sz, i32, vp, vp, sz, sz, vp, C.c_bool]),
+    "libreCuSiluMulPackQ8": (i32, [vp, sz, vp, vp, vp, vp, vp, sz, vp, sz, i32, sz, sz, vp, C.c_bool]),
+    "libreCuSiluMulGradQ8": (i32, [vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp, vp, i32, sz, sz, vp, C.c_bool]),
+    "libreCuCacheWriteQ8": (i32, [C.POINTER(CacheQ8), vp, sz, sz, vp, sz, sz, i32, vp, sz, vp, C.c_bool]),
+    "libreCuCacheReadQ8": (i32, [C.POINTER(CacheQ8), vp, sz, sz, vp, sz, sz, i32, vp, sz, vp, vp, sz, sz, sz, vp, C.c_bool]),
     "libreCuStreamWaitEvent": (i32, [vp, vp]),
     "libreCuEventQuery": (i32, [vp]),
     "libreCuEventGetTimestamp": (i32, [C.POINTER(u64), vp]),

@@ -220,6 +220,34 @@ class Stream:
     def memset_d32(self, dst, value: int, count: int):
         check(lib.libreCuMemsetD32(_ptr(dst), value, count, self.handle), "libreCuMemsetD32")
 
+    # 8-bit operators: matrices are (buffer, stride in elements), packed ones (codes, scales), cache rows (buffer,
+    # token stride, head stride)
+    def pack_q8(self, packed, src, type_: int, rows: int, cols: int, async_: bool = False):
+        check(lib.libreCuPackQ8(*map(_ptr, packed), _ptr(src[0]), src[1], type_, rows, cols, self.handle, async_), "libreCuPackQ8")
+
+    def unpack_q8(self, dst, packed, type_: int, rows: int, cols: int, async_: bool = False):
+        check(lib.libreCuUnpackQ8(_ptr(dst[0]), dst[1], type_, *map(_ptr, packed), rows, cols, self.handle, async_), "libreCuUnpackQ8")
+
+    def silu_mul_pack_q8(self, h, gate_packed, up_packed, gate, up, type_: int, rows: int, cols: int, async_: bool = False):
+        check(lib.libreCuSiluMulPackQ8(_ptr(h[0]), h[1], *map(_ptr, gate_packed), *map(_ptr, up_packed), _ptr(gate[0]), gate[1], _ptr(up[0]),
+                                       up[1], type_, rows, cols, self.handle, async_), "libreCuSiluMulPackQ8")
+
+    def silu_mul_grad_q8(self, dgate, dup, dh, gate_packed, up_packed, type_: int, rows: int, cols: int, h=None, async_: bool = False):
+        again = (None, 0) if h is None else (_ptr(h[0]), h[1])
+        check(lib.libreCuSiluMulGradQ8(_ptr(dgate[0]), dgate[1], _ptr(dup[0]), dup[1], *again, _ptr(dh[0]), dh[1], *map(_ptr, gate_packed),
+                                       *map(_ptr, up_packed), type_, rows, cols, self.handle, async_), "libreCuSiluMulGradQ8")
+
+    def cache_write_q8(self, cache: "CacheQ8", k, v, type_: int, slots, tokens: int, async_: bool = False):
+        """`v` is None for a cache of one tensor."""
+        values = (None, 0, 0) if v is None else (_ptr(v[0]), v[1], v[2])
+        check(lib.libreCuCacheWriteQ8(cache, _ptr(k[0]), k[1], k[2], *values, type_, _ptr(slots), tokens, self.handle, async_), "libreCuCacheWriteQ8")
+
+    def cache_read_q8(self, cache: "CacheQ8", k, v, type_: int, page_table, table_stride: int, lengths, first_rows, sequences: int,
+                      max_length: int, rows: int, async_: bool = False):
+        values = (None, 0, 0) if v is None else (_ptr(v[0]), v[1], v[2])
+        check(lib.libreCuCacheReadQ8(cache, _ptr(k[0]), k[1], k[2], *values, type_, _ptr(page_table), table_stride, _ptr(lengths), _ptr(first_rows),
+                                     sequences, max_length, rows, self.handle, async_), "libreCuCacheReadQ8")
+
     def wait_event(self, event: Event):
         check(lib.libreCuStreamWaitEvent(self.handle, event.handle), "libreCuStreamWaitEvent")
 

@@ -9,11 +9,13 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <functional>
 #include <map>
 #include <memory>
 #include <new>
 #include <set>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "host_logic.h"
@@ -165,7 +167,7 @@ struct LibreCUEvent_ {
 namespace lcu {
 
 struct Command {
-    enum Kind { CopyKernel, CopyEngine, Memset, Launch, EventRecord, WaitEvent, AllToAllPush, AllToAllPull, AllToAllEngines };
+    enum Kind { CopyKernel, CopyEngine, Memset, Launch, EventRecord, WaitEvent, AllToAllPush, AllToAllPull, AllToAllEngines, Convert };
     Kind kind;
     bool async = false;
     // copies / memset
@@ -187,6 +189,9 @@ struct Command {
     int rank = 0;
     std::vector<void *> peer_flags;  // lock-step engine form: every rank's flag words, own ones at [rank]
     unsigned int epoch = 0, timeout_ms = 0;
+    // 8-bit operators: the launch with its arguments, and the byte ranges that it writes
+    std::function<int(cudaStream_t)> enqueue;
+    std::vector<std::pair<const void *, size_t>> writes;
 };
 
 constexpr int kSideLanes = 8;

@@ -180,6 +180,12 @@ static libreCudaStatus_t submit(LibreCUstream st, Command &c) {
             st->main_writes.add_unknown();
             break;
         }
+        case Command::Convert:
+            LIBRECUDA_ERR_PROPAGATE(pick_lane(st, c.async, &lane));
+            if (!c.async)
+                for (const auto &w : c.writes) st->main_writes.add(w.first, w.second);
+            LCU_LCB(c.enqueue(lane));
+            break;
         case Command::Launch: {
             LIBRECUDA_ERR_PROPAGATE(pick_lane(st, c.async, &lane));
             // what a user kernel writes is unknown, and a library kernel behind it may become resident as soon as the

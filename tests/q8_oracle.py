@@ -84,3 +84,26 @@ def silu_mul_grad(g, u, dh):
     """(dgate, dup, size of dgate's terms before they are added)"""
     s, q = sigmoid(g), sigmoid(-g)
     return dh * u * s * (1 + g * q), dh * g * s, np.abs(dh * u) * s * (1 + np.abs(g) * q)
+
+
+# ---- the same for large shapes, in torch on whatever device x is on -----------------------------------------------
+
+def torch_pack(x):
+    """pack() with scales taken from the binary exponent and codes by torch's own conversion; exact for 32-bit inputs."""
+    x = x.float()
+    n = x.shape[-1]
+    full = groups(n) * GROUP
+    g = torch.nn.functional.pad(x, (0, full - n)).unflatten(-1, (-1, GROUP))
+    good = g.isfinite()
+    top = torch.where(good, g.abs(), 0).amax(-1, keepdim=True)
+    mantissa, exponent = torch.frexp(top)
+    b = torch.where(top > 0, (exponent + 118 + (mantissa > 0.875)).clamp(0, 246), 0)
+    inverse = ((254 - b) << 23).to(torch.int32).view(torch.float32)
+    codes = torch.where(good, (g * inverse).clamp(-448, 448), 0).to(torch.float8_e4m3fn).view(torch.uint8)
+    codes = torch.where(good, codes, NAN_CODE)
+    return codes.flatten(-2)[..., :n], b.squeeze(-1).to(torch.uint8)
+
+
+def torch_unpack(codes, scales):
+    s = torch.exp2(scales.double() - 127).repeat_interleave(GROUP, -1)[..., :codes.shape[-1]]
+    return codes.view(torch.float8_e4m3fn).double() * s

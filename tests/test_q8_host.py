@@ -145,3 +145,13 @@ def test_the_restatement_knows_the_format():
     assert codes[0, :5].tolist() == [0x7E, 0xB8, 0x7F, 0x7F, 0] and codes[0, 32] == 0  # 2^-140 / 2^-127 is below half the smallest code
     assert q8.scale_bytes(np.array([0.0, 448.0, np.nextafter(448, 500), 449 * 2.0 ** 119, 1.75 * 2.0 ** -119, 2.0 ** -149])).tolist() == [0, 127, 128, 246, 0, 0]
     assert q8.unpack(codes, scales)[0, 1] == -1.0
+
+
+def test_recorded_operations_need_a_stream():
+    c = cache()
+    calls = [lib.libreCuPackQ8(A, A, A, 100, 2, 3, 100, None, False), lib.libreCuUnpackQ8(A, 100, 2, A, A, 3, 100, None, False),
+             lib.libreCuSiluMulPackQ8(A, 100, A, A, A, A, A, 100, A, 100, 2, 3, 100, None, False),
+             lib.libreCuSiluMulGradQ8(A, 100, A, 100, None, 0, A, 100, A, A, A, A, 2, 3, 100, None, False),
+             lib.libreCuCacheWriteQ8(c, A, 128, 64, A, 128, 64, 2, A, 3, None, False),
+             lib.libreCuCacheReadQ8(c, A, 128, 64, A, 128, 64, 2, A, 2, A, A, 2, 32, 64, None, False)]
+    assert calls == [api.ERROR_INVALID_VALUE] * 6
