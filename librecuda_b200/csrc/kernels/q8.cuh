@@ -53,12 +53,15 @@ struct FastDiv32 {
 
 // ---- units --------------------------------------------------------------------------------------------------------
 // A unit is kValues consecutive values of a row, held by one lane; kLanes neighbouring lanes hold a group.  Its accesses come
-// in forms A.  32 or 16: bytes of an access to the wide type (the codes then in 16 or 8 bytes).  Rows at any address: in the
-// words that the address allows, 16 values (kLoose) or 8 (kLooseShort).  A loose access of a lane is a word of its own
-// stretch, so a warp touches many sectors at once; loads find them again in L1, stores do not, so kernels that store the
-// wide type at any address use the short form (unpacking 16384x8191 to bf16: 128 us against 244).
-// With A = 32 a row ends with a whole unit, with A = 16 after 8 or 16 of its values, in a loose form anywhere.
-constexpr int kLoose = 4, kLooseShort = 2;
+// in forms A.
+//   32, 16        bytes of an access to the wide type (the codes then in 16 or 8 bytes); a row ends with a whole unit, or with
+//                 8 or 16 values of one
+//   kWarp         rows at any address, ending anywhere, a warp inside one row: as kLoose, but the warp loads and stores its 512
+//                 wide values as a run of words side by side, handed over through shared memory
+//   kLoose[Short] rows at any address too short to give a warp to each: a lane fetches its 16 (8) values in the words
+//                 that the address allows.  A warp then touches many sectors at once; loads find them again in L1, stores
+//                 do not, so kernels that store the wide type use the short form.
+constexpr int kWarp = 1, kLooseShort = 2, kLoose = 4;
 template <int A>
 struct Form {
     static constexpr int kValues = A == kLooseShort ? 8 : 16;
@@ -119,6 +122,81 @@ struct Lane {
         }
     }
 };
+
+// ---- a warp's run of values -----------------------------------------------------------------------------------------
+// Up to 512 values of T that lie behind each other at any address, 16 to a lane, accessed in aligned words, lane by lane side by
+// side.  In shared memory a lane's words have one word of room behind them, so that the accesses by word and those by lane
+// both find 32 different banks.
+template <typename T>
+struct Run {
+    static constexpr int kLaneWords = 16 * (int)sizeof(T) / 4;
+    static constexpr int kSteps = kLaneWords + (sizeof(T) == 2);  // a run that starts inside a word covers one more
+    static constexpr int kScratch = 32 * (kLaneWords + 1) + 1;
+    __device__ static __forceinline__ int slot(int word) { return word + word / kLaneWords; }
+    __device__ static __forceinline__ int lane() { return threadIdx.x & 31; }
+    // values of the run, from every lane's columns to the end of the row
+    __device__ static __forceinline__ int values(int left) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)min(left, 16)); }
+
+    // p: the lane's first value.  Words that hold at least one value of the run are read whole.
+    __device__ static __forceinline__ bool odd(const T *p) { return sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(p) & 2); }
+    __device__ static __forceinline__ void load(uint32_t (&r)[kSteps], const T *p, int left) {
+        const int n = values(left), words = sizeof(T) == 2 ? (n + (int)odd(p) + 1) / 2 : n;
+        const uint32_t *q = reinterpret_cast<const uint32_t *>(p - lane() * 16 - (int)odd(p));
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) r[k] = n > 0 && k * 32 + lane() < words ? q[k * 32 + lane()] : 0u;
+    }
+    __device__ static __forceinline__ void hand_out(const uint32_t (&r)[kSteps], uint32_t (&w)[kLaneWords], const T *p, uint32_t *scratch) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+            if (k < kLaneWords || lane() == 0) scratch[slot(k * 32 + lane())] = r[k];
+        __syncwarp();
+        uint32_t t[kLaneWords + 1];
+#pragma unroll
+        for (int i = 0; i < kLaneWords; ++i) t[i] = scratch[lane() * (kLaneWords + 1) + i];
+        t[kLaneWords] = sizeof(T) == 2 ? scratch[(lane() + 1) * (kLaneWords + 1)] : 0u;
+#pragma unroll
+        for (int i = 0; i < kLaneWords; ++i) w[i] = __funnelshift_r(t[i], t[i + 1], odd(p) ? 16 : 0);
+        __syncwarp();
+    }
+    __device__ static __forceinline__ void store(const uint32_t (&w)[kLaneWords], T *p, int left, uint32_t *scratch) {
+        const int n = values(left);
+#pragma unroll
+        for (int i = 0; i < kLaneWords; ++i) scratch[lane() * (kLaneWords + 1) + i] = w[i];
+        __syncwarp();
+        T *first = p - lane() * 16;
+        if (!odd(p)) {
+            uint32_t *q = reinterpret_cast<uint32_t *>(first);
+            const int words = sizeof(T) == 2 ? n / 2 : n;
+#pragma unroll
+            for (int k = 0; k < kLaneWords; ++k)
+                if (k * 32 + lane() < words) q[k * 32 + lane()] = scratch[slot(k * 32 + lane())];
+        } else {
+            uint32_t *q = reinterpret_cast<uint32_t *>(first + 1);  // the words from the second value on
+            const int words = (n - 1) / 2;
+#pragma unroll
+            for (int k = 0; k < kLaneWords; ++k) {
+                const int word = k * 32 + lane();
+                if (word < words) q[word] = __funnelshift_r(scratch[slot(word)], scratch[slot(word + 1)], 16);
+            }
+            if (lane() == 0 && n > 0) *reinterpret_cast<uint16_t *>(first) = (uint16_t)scratch[0];
+        }
+        if constexpr (sizeof(T) == 2) {  // a last value that no word holds
+            if (lane() == 1 && n > (int)odd(p) && ((n - (int)odd(p)) & 1))
+                reinterpret_cast<uint16_t *>(first)[n - 1] = (uint16_t)(scratch[slot((n - 1) / 2)] >> (16 * ((n - 1) & 1)));
+        }
+        __syncwarp();
+    }
+};
+// a warp's scratch for runs of T
+template <typename T, int A>
+__device__ __forceinline__ uint32_t *run_scratch() {
+    if constexpr (A == kWarp) {
+        __shared__ uint32_t all[kMaxThreads / 32][Run<T>::kScratch];
+        return all[threadIdx.x / 32];
+    } else {
+        return nullptr;
+    }
+}
 
 // ---- pairs: two 32-bit operations in one instruction ----------------------------------------------------------------
 struct Pair {
@@ -182,13 +260,21 @@ struct Unit {  // as it lies in memory
     static constexpr int kWords = kValues * (int)sizeof(T) / 4;
     static constexpr int kPerWord = 4 / (int)sizeof(T);
     uint32_t w[kWords];
+    uint32_t run[A == kWarp ? Run<T>::kSteps : 1];  // kWarp: as loaded, before it is handed out
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) w[i] = 0;
     }
-    // `left` > 0: columns from the unit's first one to the end of the row.  Values behind the end are 0.
+    // `left`: columns from the unit's first one to the end of the row, 0: no unit.  Values behind the end are 0.  Every lane
+    // of the warp calls this, take() before it looks at a value, and store().
     __device__ __forceinline__ void load(const T *p, int left) {
         const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+        clear();
+        if constexpr (A == kWarp) {
+            Run<T>::load(run, p, left);
+            return;
+        }
+        if (left <= 0) return;
         if constexpr (A == 32) {
 #pragma unroll
             for (int i = 0; i < kWords; i += 8)
@@ -214,14 +300,30 @@ struct Unit {  // as it lies in memory
             for (int i = 0; i <= kWords; ++i) r[i] = 2 * i < n ? q[i] : 0u;
 #pragma unroll
             for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(r[i], r[i + 1], 16 * odd);
-            if (left < kValues) {
-#pragma unroll
-                for (int i = 0; i < kWords; ++i) w[i] = 2 * i + 1 < left ? w[i] : 2 * i < left ? w[i] & 0xffffu : 0u;
-            }
+            end_at(left);
         }
     }
-    __device__ __forceinline__ void store(T *p, int left) const {
+    __device__ __forceinline__ void end_at(int left) {
+        if (left >= kValues) return;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = i < left ? w[i] : 0u;
+            else w[i] = 2 * i + 1 < left ? w[i] : 2 * i < left ? w[i] & 0xffffu : 0u;
+        }
+    }
+    __device__ __forceinline__ void take(const T *p, int left, uint32_t *scratch) {
+        if constexpr (A == kWarp) {
+            Run<T>::hand_out(run, w, p, scratch);
+            end_at(left);
+        }
+    }
+    __device__ __forceinline__ void store(T *p, int left, uint32_t *scratch) const {
         uint32_t *q = reinterpret_cast<uint32_t *>(p);
+        if constexpr (A == kWarp) {
+            Run<T>::store(w, p, left, scratch);
+            return;
+        }
+        if (left <= 0) return;
         if constexpr (A == 32) {
 #pragma unroll
             for (int i = 0; i < kWords; i += 8)
@@ -326,6 +428,7 @@ struct Codes {  // of one unit, four to a word
     static constexpr int kWords = kValues / 4;
     uint32_t w[kWords];
     __device__ __forceinline__ void load(const uint8_t *p, int left) {
+        if (left <= 0) return;
         if constexpr (A == 32) {
             const uint4 v = ld_stream<2>(reinterpret_cast<const uint4 *>(p));
             w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
@@ -346,6 +449,7 @@ struct Codes {  // of one unit, four to a word
         }
     }
     __device__ __forceinline__ void store(uint8_t *p, int left) const {
+        if (left <= 0) return;
         if constexpr (A == 32) st_stream<2>(reinterpret_cast<uint4 *>(p), make_uint4(w[0], w[1], w[2], w[3]));
         else if constexpr (A == 16) {
             uint2 *q = reinterpret_cast<uint2 *>(p);
@@ -458,6 +562,7 @@ int with_access(int a, Fn fn) {
     switch (a) {
         case 32: return fn(std::integral_constant<int, 32>());
         case 16: return fn(std::integral_constant<int, 16>());
+        case kWarp: return fn(std::integral_constant<int, kWarp>());
         default: return fn(std::integral_constant<int, LOOSE>());
     }
 }

@@ -83,12 +83,9 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
 #pragma unroll
     for (int u = 0; u < P; ++u) {
         const uint64_t token = at.token + u * at.step;
-        slot[u] = -1;
-        x[u].clear();
-        if (at.left > 0 && token < tokens) {
-            slot[u] = slots[token];
-            x[u].load(from + u * (at.step * s.token_stride), at.left);
-        }
+        const int left = token < tokens ? at.left : 0;
+        slot[u] = left > 0 ? slots[token] : -1;
+        x[u].load(from + u * (at.step * s.token_stride), left);
     }
 #pragma unroll
     for (int u = 0; u < P; ++u) {
@@ -178,7 +175,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
             Unit<T, A> y;
 #pragma unroll
             for (int j = 0; j < Form<A>::kValues; j += 2) y.template set_pair<true>(j, c[u].pair(j, by));
-            y.store(to + u * (at.step * s.token_stride), at.left);
+            y.store(to + u * (at.step * s.token_stride), at.left, nullptr);
         }
     }
 }

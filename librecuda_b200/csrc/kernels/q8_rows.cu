@@ -13,8 +13,14 @@ namespace {
 template <int A>
 constexpr int kPassesPack = A >= 16 ? 4 : 2;
 constexpr int kPassesUnpack = 2;
-constexpr int kPassesSilu = 2;  // of each input
+template <int A>
+constexpr int kPassesSilu = A == kWarp ? 1 : 2;  // of each input
 constexpr int kPassesGrad = 1;
+// Rows at any address give each row warps of its own from here on.  Below, lanes behind the end of a row cost more than the
+// coalesced accesses save: 333 columns of bf16 take 104 us against 82 in the gated unit, 500 columns 66 against 68; 259 columns of
+// f32 take 41 us against 71 to unpack, 200 columns 65 against 52 to pack.
+template <typename T>
+constexpr size_t kWarpColumns = sizeof(T) == 4 ? 224 : 448;
 
 template <typename T>
 struct Rows {  // rows of the wide type
@@ -37,8 +43,8 @@ struct Shape {
             const uint64_t line = kMaxThreads * Form<A>::kValues, total = (uint64_t)rows * cols, lines = (total + line - 1) / line;
             return {lines, line, line / kGroup, total, Tiling::of(lines, kMaxThreads, passes)};
         }
-        const uint64_t groups = groups_of(cols);
-        return {rows, cols, groups, 0, Tiling::of(rows, groups * Form<A>::kLanes, passes)};
+        const uint64_t groups = groups_of(cols), units = groups * Form<A>::kLanes;
+        return {rows, cols, groups, 0, Tiling::of(rows, A == kWarp ? (units + 31) / 32 * 32 : units, passes)};
     }
 };
 
@@ -68,7 +74,7 @@ struct Place {
         left = last = (int)min(s.cols - column, (uint64_t)INT32_MAX);
         if (s.flat != 0 && live != 0) last = min(left, (int)(rest - (live - 1) * stride));
     }
-    __device__ __forceinline__ int columns(uint32_t pass) const { return pass + 1 == live ? last : left; }
+    __device__ __forceinline__ int columns(uint32_t pass) const { return pass >= live ? 0 : pass + 1 == live ? last : left; }
     template <typename T>
     __device__ __forceinline__ T *wide(const Rows<T> &r) const { return r.p + (row * r.stride + column); }
 };
@@ -77,32 +83,32 @@ template <typename T, int A, int P>
 __device__ __forceinline__ void pack_and_store(const Packed &out, const Shape &s, const Place<A, P> &at, uint32_t pass, const Unit<T, A> &x) {
     Codes<A> c;
     const unsigned b = pack_unit(x, c);
-    if (pass >= at.live) return;
     c.store(out.codes + at.code + pass * (at.step * s.cols), at.columns(pass));
-    if (at.leads) out.scales[at.scale + pass * (at.step * s.groups)] = (uint8_t)b;
+    if (pass < at.live && at.leads) out.scales[at.scale + pass * (at.step * s.groups)] = (uint8_t)b;
 }
 
 template <typename T, int A, int P>
 __global__ void __launch_bounds__(kMaxThreads) pack_kernel(Packed out, Rows<const T> src, Shape s) {
     pdl_launch_dependents();
     const Place<A, P> at(s);
+    uint32_t *scratch = run_scratch<T, A>();
     const T *from = at.wide(src);
     Unit<T, A> x[P];
     pdl_wait();
 #pragma unroll
-    for (uint32_t u = 0; u < P; ++u) {
-        x[u].clear();
-        if (u < at.live) x[u].load(from + u * (at.step * src.stride), at.columns(u));
-    }
+    for (uint32_t u = 0; u < P; ++u) x[u].load(from + u * (at.step * src.stride), at.columns(u));
 #pragma unroll
-    for (uint32_t u = 0; u < P; ++u)
+    for (uint32_t u = 0; u < P; ++u) {
+        x[u].take(from + u * (at.step * src.stride), at.columns(u), scratch);
         pack_and_store(out, s, at, u, x[u]);
+    }
 }
 
 template <typename T, int A, int P>
 __global__ void __launch_bounds__(kMaxThreads) unpack_kernel(Rows<T> dst, Packed in, Shape s) {
     pdl_launch_dependents();
     const Place<A, P> at(s);
+    uint32_t *scratch = run_scratch<T, A>();
     T *to = at.wide(dst);
     const uint8_t *codes = in.codes + at.code, *scales = in.scales + at.scale;
     Codes<A> c[P];
@@ -110,19 +116,17 @@ __global__ void __launch_bounds__(kMaxThreads) unpack_kernel(Rows<T> dst, Packed
     pdl_wait();
 #pragma unroll
     for (uint32_t u = 0; u < P; ++u) {
-        if (u < at.live) {
-            c[u].load(codes + u * (at.step * s.cols), at.columns(u));
-            b[u] = scales[u * (at.step * s.groups)];
-        }
+        c[u].load(codes + u * (at.step * s.cols), at.columns(u));
+        b[u] = u < at.live ? scales[u * (at.step * s.groups)] : 0;
     }
 #pragma unroll
     for (uint32_t u = 0; u < P; ++u) {
-        if (u >= at.live) break;
+        if (A != kWarp && u >= at.live) break;
         const Pair scale(scale_value(b[u]));
         Unit<T, A> y;
 #pragma unroll
         for (int j = 0; j < Form<A>::kValues; j += 2) y.template set_pair<true>(j, c[u].pair(j, scale));
-        y.store(to + u * (at.step * dst.stride), at.columns(u));
+        y.store(to + u * (at.step * dst.stride), at.columns(u), scratch);
     }
 }
 
@@ -131,29 +135,28 @@ __global__ void __launch_bounds__(kMaxThreads) silu_mul_pack_kernel(Rows<T> h, P
                                                                     Rows<const T> up, Shape s) {
     pdl_launch_dependents();
     const Place<A, P> at(s);
+    uint32_t *scratch = run_scratch<T, A>();
     const T *from_gate = at.wide(gate), *from_up = at.wide(up);
     T *to = at.wide(h);
     Unit<T, A> g[P], u[P];
     pdl_wait();
 #pragma unroll
     for (uint32_t k = 0; k < P; ++k) {
-        g[k].clear();
-        u[k].clear();
-        if (k < at.live) {
-            g[k].load(from_gate + k * (at.step * gate.stride), at.columns(k));
-            u[k].load(from_up + k * (at.step * up.stride), at.columns(k));
-        }
+        g[k].load(from_gate + k * (at.step * gate.stride), at.columns(k));
+        u[k].load(from_up + k * (at.step * up.stride), at.columns(k));
     }
 #pragma unroll
     for (uint32_t k = 0; k < P; ++k) {
-        if (k < at.live) {
+        g[k].take(from_gate + k * (at.step * gate.stride), at.columns(k), scratch);
+        u[k].take(from_up + k * (at.step * up.stride), at.columns(k), scratch);
+        if (A == kWarp || k < at.live) {
             Unit<T, A> out;
 #pragma unroll
             for (int j = 0; j < Form<A>::kValues; j += 2) {
                 const Pair x = g[k].pair(j);
                 out.template set_pair<false>(j, x * sigmoid(x).s * u[k].pair(j));
             }
-            out.store(to + k * (at.step * h.stride), at.columns(k));
+            out.store(to + k * (at.step * h.stride), at.columns(k), scratch);
         }
         pack_and_store(gate_out, s, at, k, g[k]);
         pack_and_store(up_out, s, at, k, u[k]);
@@ -165,14 +168,17 @@ __global__ void __launch_bounds__(kMaxThreads) silu_mul_grad_kernel(Rows<T> dgat
                                                                     Packed up, Shape s) {
     pdl_launch_dependents();
     const Place<A, 1> at(s);
+    uint32_t *scratch = run_scratch<T, A>();
     pdl_wait();
-    if (at.live == 0) return;
+    if (A != kWarp && at.live == 0) return;
+    const int left = at.columns(0);
     Unit<T, A> d;
     Codes<A> g, u;
-    d.load(at.wide(dh), at.last);
-    g.load(gate.codes + at.code, at.last);
-    u.load(up.codes + at.code, at.last);
-    const Pair gs(scale_value(gate.scales[at.scale])), us(scale_value(up.scales[at.scale]));
+    d.load(at.wide(dh), left);
+    g.load(gate.codes + at.code, left);
+    u.load(up.codes + at.code, left);
+    const Pair gs(scale_value(left > 0 ? gate.scales[at.scale] : 0u)), us(scale_value(left > 0 ? up.scales[at.scale] : 0u));
+    d.take(at.wide(dh), left, scratch);
     Unit<T, A> dg, du, y;
 #pragma unroll
     for (int j = 0; j < Form<A>::kValues; j += 2) {
@@ -183,9 +189,9 @@ __global__ void __launch_bounds__(kMaxThreads) silu_mul_grad_kernel(Rows<T> dgat
         dg.template set_pair<false>(j, dj * z * fma2(silu, sg.q, sg.s));
         if constexpr (AGAIN) y.template set_pair<false>(j, silu * z);
     }
-    du.store(at.wide(dup), at.last);
-    dg.store(at.wide(dgate), at.last);
-    if constexpr (AGAIN) y.store(at.wide(h), at.last);
+    du.store(at.wide(dup), left, scratch);
+    dg.store(at.wide(dgate), left, scratch);
+    if constexpr (AGAIN) y.store(at.wide(h), left, scratch);
 }
 
 // The widest accesses that are aligned in every row.  A row's codes lie behind each other, so the columns must be a multiple of
@@ -202,10 +208,11 @@ struct Fit {
         if (rows > 1 && r.stride != cols) flat = false;
     }
     void add(const Packed &p) { codes |= reinterpret_cast<uintptr_t>(p.codes); }
+    template <typename T>
     int access() const {
         if (cols % 16 == 0 && wide % 32 == 0 && codes % 16 == 0) return 32;
         if (cols % 8 == 0 && wide % 16 == 0 && codes % 8 == 0) return 16;
-        return 0;
+        return flat || cols >= kWarpColumns<T> ? kWarp : 0;
     }
     // one long row is addressed in lines that lie behind each other
     template <typename T>
@@ -253,7 +260,7 @@ extern "C" int lcb_pack_q8(void *codes, void *scales, const void *src, size_t sr
             Fit fit(rows, n);
             fit.add(in);
             fit.add(out);
-            return with_access<kLoose>(fit.access(), [&](auto a) {
+            return with_access<kLoose>(fit.template access<T>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesPack<a()>);
                 return with_passes<kPassesPack<a()>>(s.tiling.passes, [&](auto p) {
                     return launch_rows(pack_kernel<T, a(), p()>, s, stream, out, fit.lines(in, s));
@@ -275,7 +282,7 @@ extern "C" int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void 
             Fit fit(rows, n);
             fit.add(out);
             fit.add(in);
-            return with_access<kLooseShort>(fit.access(), [&](auto a) {
+            return with_access<kLooseShort>(fit.template access<T>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesUnpack);
                 return with_passes<kPassesUnpack>(s.tiling.passes, [&](auto p) {
                     return launch_rows(unpack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), in);
@@ -302,9 +309,9 @@ extern "C" int lcb_silu_mul_pack_q8(void *h, size_t h_stride, void *gate_codes, 
             fit.add(u);
             fit.add(gp);
             fit.add(upk);
-            return with_access<kLooseShort>(fit.access(), [&](auto a) {
-                const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesSilu);
-                return with_passes<kPassesSilu>(s.tiling.passes, [&](auto p) {
+            return with_access<kLooseShort>(fit.template access<T>(), [&](auto a) {
+                const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesSilu<a()>);
+                return with_passes<kPassesSilu<a()>>(s.tiling.passes, [&](auto p) {
                     return launch_rows(silu_mul_pack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), gp, upk, fit.lines(g, s), fit.lines(u, s));
                 });
             });
@@ -332,7 +339,7 @@ extern "C" int lcb_silu_mul_grad_q8(void *dgate, size_t dgate_stride, void *dup,
             fit.add(d);
             fit.add(gp);
             fit.add(upk);
-            return with_access<kLooseShort>(fit.access(), [&](auto a) {
+            return with_access<kLooseShort>(fit.template access<T>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesGrad);
                 return launch_rows(h != nullptr ? silu_mul_grad_kernel<T, a(), true> : silu_mul_grad_kernel<T, a(), false>, s, stream,
                                    fit.lines(dg, s), fit.lines(du, s), fit.lines(out, s), fit.lines(d, s), gp, upk);
