@@ -89,19 +89,21 @@ int lcb_axpb_f32(float *y, const float *x, float a, float b, size_t count, lcbSt
  * largest code; 0 when all values are zero, 246 when 448 * 2^119 < A).  A code is x / s rounded to the
  * nearest e4m3 value, ties to even, saturating at +-448.  A power of two as scale makes the division exact, so
  * a code carries exactly one rounding, the result does not depend on how it is computed, and no precision is lost
- * against a scale that uses the whole range: e4m3 is a floating format.  NaN and both infinities are stored
+ * against a scale that uses the whole range, but for values 2^-14 below their group's largest: e4m3 is a
+ * floating format.  NaN and both infinities are stored
  * as the NaN code 0x7f and do not count towards A: a bad value stays visible and spoils no neighbour.
  * The value of a code is code * s.  Bytes of scale above 246 are never written.  Where an operator returns these
  * values (lcb_cache_read_q8, lcb_unpack_q8) they are rounded to the wide type once, saturating at its largest
  * finite value (65504 in f16 may round up to the code for 65536); the NaN code gives NaN.
  *
  * `type` is an enum lcbType.  Strides are in elements of the wide type; 0 is allowed for inputs (one row read again and
- * again); the rows of an output must not overlap (1 is returned).  Wide pointers are aligned to
- * their element.  Any number of columns, any stride and alignment give the same result; rows whose number of columns,
- * address and stride are multiples of 16 elements (32 bytes) are fastest, see the kernels.  Inputs and
- * outputs must not overlap, except that an output of the two silu_mul operators may be exactly an input's rows
- * (same address and stride).  No workspace is used: calls on several streams may run at once, and a call may be
- * captured into a CUDA graph (make one call, or lcb_preload, on the device first).  A call with nothing to do returns 0.
+ * again); the rows of an output must not overlap (1 is returned).  Wide pointers are aligned to their element.  Any number of
+ * columns, any stride and alignment give the same result; fastest are rows whose number of columns and stride are
+ * multiples of 16 elements, at addresses that are multiples of 32 bytes (codes: 16), nearly as fast multiples of half of that.
+ * Outputs must not overlap each other (1 is returned where two begin at one address) nor an input, except that a
+ * wide output of the two silu_mul operators may be exactly an input's rows (same address and stride).  No workspace is
+ * used: calls on several streams may run at once, and a call may be captured into a CUDA graph.  A call with nothing to
+ * do returns 0.
  * ref: none (the reference has no operation that changes a format; driverapi/include/librecuda.h:37-114). */
 
 /* Writes `tokens` rows of keys and values into a paged cache, quantising them: the row of token t, head h,

@@ -16,8 +16,7 @@ namespace {
 template <int A>
 constexpr int kPassesWrite = A >= 16 ? 4 : 2;
 constexpr int kPassesRead = 2;
-constexpr int kRunTiles = 4;  // tiles that a CTA of a read takes, at most
-constexpr int kRunWaves = 4;
+constexpr int kRunTiles = 4, kRunWaves = 4, kMostWaves = 64;  // tiles that a CTA of a read takes, see its launcher
 
 template <typename T>
 struct Side {  // keys or values
@@ -286,9 +285,11 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         return by_sides<kLooseShort, T>(*cache, kw, vw, max_length, rows, sequences, [](auto) { return kPassesRead; }, [&](auto a, auto p, const Side<T> &ks, const Side<T> &vs) {
-            // as many tiles to a CTA as leave the GPU kRunWaves grids of resident CTAs
-            const uint64_t all = ((uint64_t)ks.blocks + vs.blocks) * sequences, want = Tiling::resident_ctas() * kRunWaves;
-            const uint32_t tiles = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(all / want, 1), kRunTiles);
+            // Up to kRunTiles tiles to a CTA while that leaves the GPU kRunWaves grids of resident CTAs, and more of them
+            // where the grid would have more than kMostWaves: max_length may be far above the lengths.
+            const uint64_t all = ((uint64_t)ks.blocks + vs.blocks) * sequences, wave = Tiling::resident_ctas();
+            const uint32_t tiles = (uint32_t)std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(all / (wave * kRunWaves), 1), kRunTiles),
+                                                                std::min<uint64_t>(all / (wave * kMostWaves), 0x7fffffffu));
             Side<T> kr = ks, vr = vs;
             auto runs = [&](Side<T> &s) {
                 if (s.blocks == 0) return;
@@ -298,7 +299,7 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
             runs(kr);
             runs(vr);
             const uint64_t each = (uint64_t)kr.blocks + vr.blocks;
-            if (ks.blocks > 0x7fffffffu || vs.blocks > 0x7fffffffu || sequences > 0x7fffffffu / each) return 1;
+            if (ks.blocks > 0x7fffffffu || vs.blocks > 0x7fffffffu || each > 0x7fffffffu || sequences > 0x7fffffffu / each) return 1;
             const Sequences q{page_table, lengths, first_rows, table_stride, rows, (uint32_t)max_length, tiles, FastDiv32::of((uint32_t)each)};
             const unsigned threads = std::max(ks.tiling.threads, vs.tiling.threads);
             return launch_kernel(cache_read_kernel<T, a(), p()>, (unsigned)(each * sequences), threads, 0, static_cast<cudaStream_t>(stream), kr, vr,

@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "lcb200_types.h"
 
 namespace lcb {
@@ -28,6 +30,13 @@ inline bool product_ok(size_t a, size_t b, size_t c, size_t d) {  // a * b * c *
     return !__builtin_mul_overflow(a, b, &p) && !__builtin_mul_overflow(p, c, &p) && !__builtin_mul_overflow(p, d, &p) && !(p >> 62);
 }
 
+// outputs that begin at the same address write over each other (NULL: left out)
+inline bool apart(std::initializer_list<const void *> outputs) {
+    for (auto a = outputs.begin(); a != outputs.end(); ++a)
+        for (auto b = a + 1; b != outputs.end(); ++b)
+            if (*a != nullptr && *a == *b) return false;
+    return true;
+}
 // rows of an output: none may overlap another
 inline bool rows_apart(size_t rows, size_t stride, size_t cols) { return rows <= 1 || stride >= cols; }
 // the same for rows (t, h), whichever of the two is the outer dimension
@@ -50,15 +59,15 @@ inline bool packed_matrix_ok(const void *codes, const void *scales, size_t rows,
 inline bool pack_ok(const void *codes, const void *scales, const void *wide, size_t stride, int type, size_t rows, size_t cols, bool wide_is_output) {
     if (!type_ok(type)) return false;
     if (rows == 0 || cols == 0) return true;
-    return packed_matrix_ok(codes, scales, rows, cols) && wide_matrix_ok(wide, stride, type, rows, cols, wide_is_output);
+    return codes != scales && codes != wide && scales != wide && packed_matrix_ok(codes, scales, rows, cols) && wide_matrix_ok(wide, stride, type, rows, cols, wide_is_output);
 }
 
 inline bool silu_pack_ok(const void *h, size_t h_stride, const void *gate_codes, const void *gate_scales, const void *up_codes, const void *up_scales,
                          const void *gate, size_t gate_stride, const void *up, size_t up_stride, int type, size_t rows, size_t cols) {
     if (!type_ok(type)) return false;
     if (rows == 0 || cols == 0) return true;
-    return packed_matrix_ok(gate_codes, gate_scales, rows, cols) && packed_matrix_ok(up_codes, up_scales, rows, cols) &&
-           wide_matrix_ok(h, h_stride, type, rows, cols, true) && wide_matrix_ok(gate, gate_stride, type, rows, cols, false) &&
+    return apart({h, gate_codes, gate_scales, up_codes, up_scales}) && packed_matrix_ok(gate_codes, gate_scales, rows, cols) &&
+           packed_matrix_ok(up_codes, up_scales, rows, cols) && wide_matrix_ok(h, h_stride, type, rows, cols, true) && wide_matrix_ok(gate, gate_stride, type, rows, cols, false) &&
            wide_matrix_ok(up, up_stride, type, rows, cols, false);
 }
 inline bool silu_grad_ok(const void *dgate, size_t dgate_stride, const void *dup, size_t dup_stride, const void *h, size_t h_stride, const void *dh,
@@ -66,7 +75,7 @@ inline bool silu_grad_ok(const void *dgate, size_t dgate_stride, const void *dup
                          size_t rows, size_t cols) {
     if (!type_ok(type)) return false;
     if (rows == 0 || cols == 0) return true;
-    return packed_matrix_ok(gate_codes, gate_scales, rows, cols) && packed_matrix_ok(up_codes, up_scales, rows, cols) &&
+    return apart({dgate, dup, h}) && packed_matrix_ok(gate_codes, gate_scales, rows, cols) && packed_matrix_ok(up_codes, up_scales, rows, cols) &&
            wide_matrix_ok(dgate, dgate_stride, type, rows, cols, true) && wide_matrix_ok(dup, dup_stride, type, rows, cols, true) &&
            (h == nullptr || wide_matrix_ok(h, h_stride, type, rows, cols, true)) && wide_matrix_ok(dh, dh_stride, type, rows, cols, false);
 }
@@ -105,7 +114,7 @@ inline bool cache_write_ok(const lcbCacheQ8 *c, const void *k, size_t kts, size_
                            const int64_t *slots, size_t tokens) {
     if (!cache_ok(c) || !type_ok(type)) return false;
     if (tokens == 0) return true;
-    return slots != nullptr && aligned(slots, 8) && cache_rows_ok(*c, k, kts, khs, v, vts, vhs, type, tokens, false);
+    return apart({c->k_codes, c->k_scales, c->v_codes, c->v_scales}) && slots != nullptr && aligned(slots, 8) && cache_rows_ok(*c, k, kts, khs, v, vts, vhs, type, tokens, false);
 }
 inline bool cache_read_ok(const lcbCacheQ8 *c, const void *k, size_t kts, size_t khs, const void *v, size_t vts, size_t vhs, int type,
                           const int32_t *table, size_t table_stride, const int32_t *lengths, const int64_t *first_rows, size_t sequences,
@@ -120,7 +129,7 @@ inline bool cache_read_ok(const lcbCacheQ8 *c, const void *k, size_t kts, size_t
     if (!aligned(table, 4) || !aligned(lengths, 4) || !aligned(first_rows, 8) || (rows >> 62)) return false;
     return product_ok(sequences, max_length, c->heads, groups_of(c->k_dim) * 32) &&
            product_ok(sequences, max_length, c->heads, groups_of(c->v_dim) * 32) &&
-           cache_rows_ok(*c, k, kts, khs, v, vts, vhs, type, rows, true);
+           (c->v_dim == 0 || apart({k, v})) && cache_rows_ok(*c, k, kts, khs, v, vts, vhs, type, rows, true);
 }
 
 }  // namespace lcb

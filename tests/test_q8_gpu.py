@@ -7,6 +7,10 @@ argument's rounding, 1 + e adds u, the quotient at most 4 u, a product u.  So si
 chain sigmoid, g * sigmoid, * (1 - sigmoid), the sum and two products: 13 + 12 + 1 + 3 = 29 u of the terms' size, below
 2^-19.  The result is rounded to its type by at most eps / 2 of itself, or half its smallest subnormal.  Below
 exp(-87) the sigmoid itself is subnormal or zero in 32 bits: 2^-126 of the factors is added for that."""
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -15,6 +19,7 @@ import q8_oracle as q8
 from librecuda_b200 import api
 
 pytestmark = pytest.mark.gpu
+ROOT = Path(__file__).resolve().parent.parent
 lib = api.lib
 KINDS = ["f32", "f16", "bf16"]
 GUARD = 0xC5
@@ -240,18 +245,19 @@ def test_gradients_agree_with_differences():
     assert np.all(np.abs(du.double().cpu().numpy() - by_u) <= bound)
 
 
-@pytest.mark.parametrize("cols", [512, 70])
-def test_outputs_may_be_the_rows_of_an_input(cols):
-    rows = 40
-    g, u, d = (torch.randn(rows, cols, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(40, 512), (40, 70), (40, 1001), (40, 1416), (1, 5003), (6000, 600), (2000, 1003)])
+def test_outputs_may_be_the_rows_of_an_input(rows, cols, kind):
+    code = q8.TYPE_CODES[kind]
+    g, u, d = (torch.randn(rows, cols, device="cuda").to(q8.TORCH_TYPES[kind]) for _ in range(3))
     packs = [torch.empty(rows, n, dtype=torch.uint8, device="cuda") for n in (cols, q8.groups(cols)) * 2]
     ptrs = [p.data_ptr() for p in packs]
 
     def forward(h, g, u):
-        ok(lib.lcb_silu_mul_pack_q8(h.data_ptr(), cols, *ptrs, g.data_ptr(), cols, u.data_ptr(), cols, 2, rows, cols, current()))
+        ok(lib.lcb_silu_mul_pack_q8(h.data_ptr(), cols, *ptrs, g.data_ptr(), cols, u.data_ptr(), cols, code, rows, cols, current()))
 
     def backward(dg, du, dh):
-        ok(lib.lcb_silu_mul_grad_q8(dg.data_ptr(), cols, du.data_ptr(), cols, None, 0, dh.data_ptr(), cols, *ptrs, 2, rows, cols, current()))
+        ok(lib.lcb_silu_mul_grad_q8(dg.data_ptr(), cols, du.data_ptr(), cols, None, 0, dh.data_ptr(), cols, *ptrs, code, rows, cols, current()))
 
     h, dg, du = (torch.empty_like(g) for _ in range(3))
     forward(h, g, u)
@@ -481,6 +487,35 @@ def test_a_decoding_step_replayed_from_a_graph_sees_new_inputs():
                 assert torch.equal(out[32 * b:32 * b + t + 1].cpu(), want)
                 assert bool((out[32 * b + t + 1:32 * b + 32] == 0).all())
     assert api.device_error_word() == 0
+
+
+def test_the_first_call_of_a_process_may_be_captured(tmp_path):
+    script = tmp_path / "first.py"
+    script.write_text(f"""
+import sys
+sys.path[:0] = [{str(ROOT)!r}, {str(ROOT / "tests")!r}]
+import torch
+import q8_oracle as q8
+from librecuda_b200 import api
+x = torch.randn(100, 256, device="cuda")
+codes, scales = (torch.zeros(100, n, dtype=torch.uint8, device="cuda") for n in (256, 8))
+pool = [torch.zeros(128 * 256, dtype=torch.uint8, device="cuda") for _ in range(2)]
+slots = torch.arange(100, device="cuda")
+cache = api.CacheQ8(pool[0].data_ptr(), pool[1].data_ptr(), None, None, 8, 16, 1, 256, 0, 0)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    stream = torch.cuda.current_stream().cuda_stream
+    assert api.lib.lcb_pack_q8(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), 256, 0, 100, 256, stream) == 0
+    assert api.lib.lcb_cache_write_q8(cache, x.data_ptr(), 256, 256, None, 0, 0, 0, slots.data_ptr(), 100, stream) == 0
+graph.replay()
+torch.cuda.synchronize()
+want = q8.torch_pack(x)
+assert torch.equal(codes, want[0]) and torch.equal(scales, want[1]) and torch.equal(pool[0][:25600].view(100, 256), want[0])
+print("first call captured")
+""")
+    run = subprocess.run([sys.executable, str(script)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "first call captured" in run.stdout, run.stderr[-2000:]
 
 
 def test_two_streams_at_once_give_what_each_gives_alone():

@@ -12,11 +12,12 @@ from librecuda_b200 import api
 
 lib = N.lib
 A = 1 << 20  # an address that nothing reads: every call here is refused, or has nothing to do
+B, D, E, F, G = (A * i for i in range(2, 7))
 BIG = 1 << 62
 
 
 def cache(**over):
-    fields = dict(k_codes=A, k_scales=A, v_codes=A, v_scales=A, pages=4, page_tokens=16, heads=2, k_dim=64, v_dim=64, order=0)
+    fields = dict(k_codes=A, k_scales=B, v_codes=D, v_scales=E, pages=4, page_tokens=16, heads=2, k_dim=64, v_dim=64, order=0)
     fields.update(over)
     return api.CacheQ8(**fields)
 
@@ -25,7 +26,7 @@ def write(c=None, k=A, kts=128, khs=64, v=A, vts=128, vhs=64, kind=2, slots=A, t
     return lib.lcb_cache_write_q8(cache() if c is None else c, k, kts, khs, v, vts, vhs, kind, slots, tokens, None)
 
 
-def read(c=None, k=A, kts=128, khs=64, v=A, vts=128, vhs=64, kind=2, table=A, stride=2, lengths=A, first=A, n=2, longest=32, rows=64):
+def read(c=None, k=A, kts=128, khs=64, v=B, vts=128, vhs=64, kind=2, table=A, stride=2, lengths=A, first=A, n=2, longest=32, rows=64):
     return lib.lcb_cache_read_q8(cache() if c is None else c, k, kts, khs, v, vts, vhs, kind, table, stride, lengths, first, n, longest,
                                  rows, None)
 
@@ -72,11 +73,11 @@ def test_a_cache_call_with_nothing_to_do_returns_at_once():
     assert lib.lcb_cache_write_q8(None, A, 1, 1, A, 1, 1, 0, A, 1, None) == 1
 
 
-def pack(codes=A, scales=A, x=A, stride=100, kind=2, rows=3, cols=100):
+def pack(codes=A, scales=B, x=D, stride=100, kind=2, rows=3, cols=100):
     return lib.lcb_pack_q8(codes, scales, x, stride, kind, rows, cols, None)
 
 
-def unpack(y=A, stride=100, kind=2, codes=A, scales=A, rows=3, cols=100):
+def unpack(y=A, stride=100, kind=2, codes=B, scales=D, rows=3, cols=100):
     return lib.lcb_unpack_q8(y, stride, kind, codes, scales, rows, cols, None)
 
 
@@ -93,11 +94,11 @@ def test_a_bad_unpack_is_refused(over):
     assert unpack(**over) == 1
 
 
-def silu(h=A, hs=100, gc=A, gs=A, uc=A, us=A, g=A, gst=100, u=A, ust=100, kind=2, rows=3, cols=100):
+def silu(h=A, hs=100, gc=B, gs=D, uc=E, us=F, g=G, gst=100, u=G, ust=100, kind=2, rows=3, cols=100):
     return lib.lcb_silu_mul_pack_q8(h, hs, gc, gs, uc, us, g, gst, u, ust, kind, rows, cols, None)
 
 
-def grad(dg=A, dgs=100, du=A, dus=100, h=A, hs=100, dh=A, dhs=100, gc=A, gs=A, uc=A, us=A, kind=2, rows=3, cols=100):
+def grad(dg=A, dgs=100, du=B, dus=100, h=D, hs=100, dh=E, dhs=100, gc=A, gs=A, uc=A, us=A, kind=2, rows=3, cols=100):
     return lib.lcb_silu_mul_grad_q8(dg, dgs, du, dus, h, hs, dh, dhs, gc, gs, uc, us, kind, rows, cols, None)
 
 
@@ -112,6 +113,14 @@ def test_a_bad_silu_mul_pack_is_refused(over):
                                   dict(hs=50), dict(cols=BIG)], ids=str)
 def test_a_bad_silu_mul_grad_is_refused(over):
     assert grad(**over) == 1
+
+
+def test_outputs_at_one_address_are_refused():
+    assert pack(codes=B) == 1 and pack(x=A) == 1 and unpack(y=B) == 1 and unpack(codes=D) == 1
+    assert silu(gc=A) == 1 and silu(uc=B) == 1 and silu(us=D) == 1
+    assert grad(du=A) == 1 and grad(h=A) == 1 and grad(h=B) == 1
+    assert write(cache(v_codes=A)) == 1 and write(cache(v_scales=B)) == 1 and write(cache(k_scales=A)) == 1
+    assert read(v=A) == 1
 
 
 def test_an_empty_matrix_is_nothing_to_do():

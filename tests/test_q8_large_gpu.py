@@ -155,3 +155,78 @@ def test_large_caches(kind, heads, k_dim, v_dim, page, heads_first):
         assert torch.equal(out[:total].nan_to_num(nan=0.0), want.nan_to_num(nan=0.0)) and torch.equal(out[:total].isnan(), want.isnan())
         assert bool((out[total:] == 3.0).all())
     assert api.device_error_word() == 0
+
+
+@pytest.mark.gpu
+def test_a_bound_far_above_the_lengths():
+    # the grid is sized for max_length; sequences this short use one page of it each
+    sequences, longest, page, dim = 4096, 1 << 20, 1024, 32
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    lengths = torch.randint(0, 41, (sequences,), generator=gen, device="cuda")
+    lengths[7] = 1024
+    total = int(lengths.sum())
+    first = lengths.cumsum(0) - lengths
+    table = torch.full((sequences, longest // page), -1, dtype=torch.int32, device="cuda")
+    table[:, 0] = torch.randperm(sequences, generator=gen, device="cuda").int()
+    codes = torch.randint(0, 127, (sequences, page, 1, dim), generator=gen, device="cuda", dtype=torch.uint8)
+    scales = torch.randint(100, 140, (sequences, page, 1, 1), generator=gen, device="cuda", dtype=torch.uint8)
+    cache = api.CacheQ8(codes.data_ptr(), scales.data_ptr(), None, None, sequences, page, 1, dim, 0, 0)
+    out = torch.full((total + 1, 1, dim), 3.0, device="cuda")
+    ok(lib.lcb_cache_read_q8(cache, out.data_ptr(), dim, dim, None, 0, 0, 0, table.data_ptr(), table.stride(0), lengths.int().data_ptr(), first.data_ptr(),
+                             sequences, longest, total + 1, current()))
+    which = torch.repeat_interleave(lengths)
+    position = torch.arange(total, device="cuda") - first[which]
+    at = table[which, 0].long()
+    assert torch.equal(out[:total], q8.torch_unpack(codes[at, position], scales[at, position]).float())
+    assert bool((out[total] == 3).all()) and api.device_error_word() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", [api.CACHE_TOKENS_FIRST, api.CACHE_HEADS_FIRST])
+def test_slots_beyond_32_bits(order):
+    page, pages = 1 << 16, (1 << 16) + 3
+    codes = torch.full((pages * page * 2,), 0xC5, dtype=torch.uint8, device="cuda")
+    scales = torch.full((pages * page * 2,), 0xC5, dtype=torch.uint8, device="cuda")
+    cache = api.CacheQ8(codes.data_ptr(), scales.data_ptr(), None, None, pages, page, 2, 1, 0, order)
+    slots = torch.tensor([0, 5, page - 1, 2**32 - 1, 2**32, 2**32 + 70_000, pages * page - 1, -2**40], device="cuda")
+    x = torch.arange(1, 17, device="cuda", dtype=torch.float32).view(8, 2, 1)
+    ok(lib.lcb_cache_write_q8(cache, x.data_ptr(), 2, 1, None, 0, 0, 0, slots.data_ptr(), 8, current()))
+    want = q8.torch_pack(x)
+    for t in range(7):
+        p, o = int(slots[t]) // page, int(slots[t]) % page
+        for h in range(2):
+            row = (p * 2 + h) * page + o if order else (p * page + o) * 2 + h
+            assert int(codes[row]) == int(want[0][t, h, 0]) and int(scales[row]) == int(want[1][t, h, 0])
+    assert sum(int((c != 0xC5).sum()) for c in codes.chunk(8)) == 14
+    assert api.device_error_word() == 0
+    # the last page read back
+    table = torch.tensor([[pages - 1]], dtype=torch.int32, device="cuda")
+    lengths, first = torch.tensor([page], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.long, device="cuda")
+    codes.view(pages, -1)[pages - 1] = torch.where(codes.view(pages, -1)[pages - 1] == 0xC5, 0, codes.view(pages, -1)[pages - 1])
+    out = torch.zeros(page, 2, device="cuda")
+    ok(lib.lcb_cache_read_q8(cache, out.data_ptr(), 2, 1, None, 0, 0, 0, table.data_ptr(), 1, lengths.data_ptr(), first.data_ptr(), 1, page, page, current()))
+    assert out[-1].tolist() == [13.0, 14.0] and int((out != 0).sum()) == 2
+    del codes, scales
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_rows_beyond_32_bits():
+    rows = 2**32 + 1000
+    x = torch.ones(rows, dtype=torch.bfloat16, device="cuda")
+    for lo in (0, 2**31 - 40, 2**32 - 40, rows - 100):
+        x[lo:lo + 100] = torch.arange(100, device="cuda", dtype=torch.bfloat16) - 50
+    codes, scales = torch.zeros(rows, dtype=torch.uint8, device="cuda"), torch.zeros(rows, dtype=torch.uint8, device="cuda")
+    ok(lib.lcb_pack_q8(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), 1, 2, rows, 1, current()))
+    for lo in range(0, rows, 1 << 28):
+        c, s = q8.torch_pack(x[lo:lo + (1 << 28)].view(-1, 1))
+        assert torch.equal(codes[lo:lo + (1 << 28)], c.view(-1)) and torch.equal(scales[lo:lo + (1 << 28)], s.view(-1))
+        del c, s
+    x.zero_()
+    ok(lib.lcb_unpack_q8(x.data_ptr(), 1, 2, codes.data_ptr(), scales.data_ptr(), rows, 1, current()))
+    kept = q8.torch_unpack(*q8.torch_pack((torch.arange(100, device="cuda") - 50).view(-1, 1))).view(-1).bfloat16()  # e4m3 keeps four bits
+    for lo in (0, 2**31 - 40, 2**32 - 40, rows - 100):
+        assert torch.equal(x[lo:lo + 100], kept)
+    assert float(x[1000:2**31 - 1000:65537].min()) == 1.0
+    del x, codes, scales
+    torch.cuda.empty_cache()
