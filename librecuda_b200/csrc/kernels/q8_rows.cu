@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kMaxThreads) unpack_kernel(Rows<T> dst, Packed
 }
 
 template <typename T, int A, int P>
-__global__ void __launch_bounds__(kMaxThreads, A == kWarp ? 6 : 1) silu_mul_pack_kernel(Rows<T> h, Packed gate_out, Packed up_out, Rows<const T> gate,
+__global__ void __launch_bounds__(kMaxThreads, A == kWarp ? 6 : 0) silu_mul_pack_kernel(Rows<T> h, Packed gate_out, Packed up_out, Rows<const T> gate,
                                                                     Rows<const T> up, Shape s) {
     pdl_launch_dependents();
     const Place<A, P> at(s);
