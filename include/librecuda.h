@@ -7,8 +7,8 @@
 // reference declaration (header line) and implementation (driverapi/src/librecuda.cpp lines) it
 // stands in for.
 //
-// Part 2 is additive: memset, direction-checked copies, cross-stream event waits and the multi-GPU
-// (peer / partitioned / all-to-all / broadcast / IPC) entry points.  The reference has no counterpart
+// Part 2 is additive: memset, direction-checked copies, copies that change the number format (8-bit caches and
+// checkpoints), cross-stream event waits and the multi-GPU (peer / partitioned / all-to-all / broadcast / IPC) entry points.  The reference has no counterpart
 // for any of them; they follow the same conventions (status return, stream-recorded execution,
 // validation line on stderr, no exceptions across the ABI).
 //
