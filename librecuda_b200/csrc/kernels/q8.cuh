@@ -58,13 +58,14 @@ struct FastDiv32 {
 //                 8 or 16 values of one
 //   kWarp         rows at any address, ending anywhere, a warp inside one row: as kLoose, but the warp loads and stores its 512
 //                 wide values as a run of words side by side, handed over through shared memory
-//   kLoose[Short] rows at any address too short to give a warp to each: a lane fetches its 16 (8) values in the words
-//                 that the address allows.  A warp then touches many sectors at once; loads find them again in L1, stores
-//                 do not, so kernels that store the wide type use the short form.
-constexpr int kWarp = 1, kLooseShort = 2, kLoose = 4;
+//   kLoose, kLooseShort, kLooseTiny
+//                 rows at any address too short to give a warp to each: a lane fetches its 16, 8 or 4 values in the words that
+//                 the address allows.  A warp then touches many sectors at once; loads find them again in L1, stores do
+//                 not, so what a kernel moves decides how many values serve it best.
+constexpr int kWarp = 1, kLooseShort = 2, kLooseTiny = 3, kLoose = 4;
 template <int A>
 struct Form {
-    static constexpr int kValues = A == kLooseShort ? 8 : 16;
+    static constexpr int kValues = A == kLooseTiny ? 4 : A == kLooseShort ? 8 : 16;
     static constexpr int kLanes = kGroup / kValues;
 };
 

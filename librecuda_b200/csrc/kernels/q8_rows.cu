@@ -34,10 +34,17 @@ template <int A>
 constexpr int kPassesSilu = A == kWarp ? 1 : 2;
 constexpr int kPassesGrad = 1;
 // Rows at any address give each row warps of its own from here on.  Below, lanes behind the end of a row cost more than the
-// coalesced accesses save: 333 columns of bf16 take 104 us against 82 in the gated unit, 500 columns 66 against 68; 259 columns of
-// f32 take 41 us against 71 to unpack, 200 columns 65 against 52 to pack.
+// side-by-side accesses save.  16-bit types: 333 columns of bf16 take 104 us against 82 in the gated unit, 500 columns 66 against
+// 68.  f32 with packing: 333 columns 44 us against 40 to pack, 500 columns 30 against 37; without: 259 columns 41 us against 60 to
+// unpack, 200 columns equal.
+template <typename T, bool PACKS>
+constexpr size_t kWarpColumns = sizeof(T) == 2 ? 448 : PACKS ? 400 : 224;
+// Rows that stay below: values per lane.  Loads of 32-bit values share sectors less, so fewer to a lane; stores still fewer (100
+// columns of f32: pack 35 us with 8, 45 with 16, 40 with 4; unpack 48 with 4, 74 with 8; the 16-bit types the other way round).
 template <typename T>
-constexpr size_t kWarpColumns = sizeof(T) == 4 ? 224 : 448;
+constexpr int kPackForm = sizeof(T) == 4 ? kLooseShort : kLoose;
+template <typename T>
+constexpr int kStoreForm = sizeof(T) == 4 ? kLooseTiny : kLooseShort;
 
 template <typename T>
 struct Rows {  // rows of the wide type
@@ -225,11 +232,11 @@ struct Fit {
         if (rows > 1 && r.stride != cols) flat = false;
     }
     void add(const Packed &p) { codes |= reinterpret_cast<uintptr_t>(p.codes); }
-    template <typename T>
+    template <typename T, bool PACKS>
     int access() const {
         if (cols % 16 == 0 && wide % 32 == 0 && codes % 16 == 0) return 32;
         if (cols % 8 == 0 && wide % 16 == 0 && codes % 8 == 0) return 16;
-        return flat || cols >= kWarpColumns<T> ? kWarp : 0;
+        return flat || cols >= kWarpColumns<T, PACKS> ? kWarp : 0;
     }
     // one long row is addressed in lines that lie behind each other
     template <typename T>
@@ -277,7 +284,7 @@ extern "C" int lcb_pack_q8(void *codes, void *scales, const void *src, size_t sr
             Fit fit(rows, n);
             fit.add(in);
             fit.add(out);
-            return with_access<kLoose>(fit.template access<T>(), [&](auto a) {
+            return with_access<kPackForm<T>>(fit.template access<T, true>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesPack<a()>);
                 return with_passes<kPassesPack<a()>>(s.tiling.passes, [&](auto p) {
                     return launch_rows(pack_kernel<T, a(), p()>, s, stream, out, fit.lines(in, s));
@@ -299,7 +306,7 @@ extern "C" int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void 
             Fit fit(rows, n);
             fit.add(out);
             fit.add(in);
-            return with_access<kLooseShort>(fit.template access<T>(), [&](auto a) {
+            return with_access<kStoreForm<T>>(fit.template access<T, false>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesUnpack);
                 return with_passes<kPassesUnpack>(s.tiling.passes, [&](auto p) {
                     return launch_rows(unpack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), in);
@@ -326,7 +333,7 @@ extern "C" int lcb_silu_mul_pack_q8(void *h, size_t h_stride, void *gate_codes, 
             fit.add(u);
             fit.add(gp);
             fit.add(upk);
-            return with_access<kLooseShort>(fit.template access<T>(), [&](auto a) {
+            return with_access<kStoreForm<T>>(fit.template access<T, true>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesSilu<a()>);
                 return with_passes<kPassesSilu<a()>>(s.tiling.passes, [&](auto p) {
                     return launch_rows(silu_mul_pack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), gp, upk, fit.lines(g, s), fit.lines(u, s));
@@ -356,7 +363,7 @@ extern "C" int lcb_silu_mul_grad_q8(void *dgate, size_t dgate_stride, void *dup,
             fit.add(d);
             fit.add(gp);
             fit.add(upk);
-            return with_access<kLooseShort>(fit.template access<T>(), [&](auto a) {
+            return with_access<kStoreForm<T>>(fit.template access<T, false>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesGrad);
                 return launch_rows(h != nullptr ? silu_mul_grad_kernel<T, a(), true> : silu_mul_grad_kernel<T, a(), false>, s, stream,
                                    fit.lines(dg, s), fit.lines(du, s), fit.lines(out, s), fit.lines(d, s), gp, upk);
