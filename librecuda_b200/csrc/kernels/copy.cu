@@ -21,6 +21,7 @@
 //  * alltoall_kernel     one launch that moves every chunk of an all-to-all between this GPU and all its
 //                       peers (the copy fused with the exchange), by remote loads (pull) or stores (push).
 #include <cstdio>
+#include <mutex>
 
 #include "common.cuh"
 #include "lcb200_kernels.h"
@@ -1461,18 +1462,19 @@ int setup_error_mirror() {
 
 // Where kernels of the other sources raise bits of the same word: the device addresses, looked up once per device.
 int error_sink(ErrorSink *out) {
+    static std::mutex guard;
     static ErrorSink cached[64] = {};
     int dev = -1;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return (int)err;
     if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
-    if (cached[dev].mirror == nullptr) {
+    const std::lock_guard<std::mutex> lock(guard);
+    if (cached[dev].word == nullptr) {
         void *word = nullptr, *mirror = nullptr;
-        err = cudaGetSymbolAddress(&word, g_error_word);
-        if (err == cudaSuccess) err = cudaGetSymbolAddress(&mirror, g_error_mirror);
+        err = cudaGetSymbolAddress(&mirror, g_error_mirror);
+        if (err == cudaSuccess) err = cudaGetSymbolAddress(&word, g_error_word);
         if (err != cudaSuccess) return (int)err;
-        cached[dev].word = static_cast<unsigned int *>(word);
-        cached[dev].mirror = static_cast<unsigned int **>(mirror);
+        cached[dev] = {static_cast<unsigned int *>(word), static_cast<unsigned int **>(mirror)};
     }
     *out = cached[dev];
     return 0;

@@ -163,14 +163,14 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
             const uint32_t entry = pool.page_tokens32.divmod(p, offset[u]);
             page[u] = p < n ? table[entry] : 0;
         }
-        const int64_t row = first_row + (int64_t)token;
+        const uint64_t row = (uint64_t)first_row + token;  // a negative first row wraps to where no row is
         Codes<A> c[P];
         unsigned scale[P];
         bool live[P];
 #pragma unroll
         for (int u = 0; u < P; ++u) {
             live[u] = at.left > 0 && token + u * at.step < n;
-            if (live[u] && ((uint32_t)page[u] >= pool.pages || (uint64_t)(row + (int64_t)(u * at.step)) >= q.rows)) {
+            if (live[u] && ((uint32_t)page[u] >= pool.pages || row + u * at.step >= q.rows)) {
                 if (at.first) raise_error(errors, kErrIndexRange);
                 live[u] = false;
             }
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
                 scale[u] = scales[(uint32_t)page[u] * s.page_scales + (uint64_t)offset[u] * s.token_scales];
             }
         }
-        T *to = s.wide + ((uint64_t)row * s.token_stride + at.wide);  // no access before the row is checked
+        T *to = s.wide + (row * s.token_stride + at.wide);  // no access before the row is checked
 #pragma unroll
         for (int u = 0; u < P; ++u) {
             if (!live[u]) continue;

@@ -403,7 +403,8 @@ def test_indices_out_of_range_are_skipped_and_reported(ctx):
     good_table, good_lengths, good_first = [[0, 1], [2, 3]], [20, 17], [0, 20]
     cases = [("table", [[0, 4], [2, 3]], {*range(0, 16), *range(20, 37)}), ("table", [[0, 1], [-1, 3]], {*range(20), 36}),
              ("lengths", [33, 17], {*range(32), *range(32, 37)}), ("lengths", [-1, 17], {*range(20, 37)}),
-             ("first", [0, 30], {*range(20), *range(30, 40)}), ("first", [-5, 20], {*range(0, 15), *range(20, 37)})]
+             ("first", [0, 30], {*range(20), *range(30, 40)}), ("first", [-5, 20], {*range(0, 15), *range(20, 37)}),
+             ("first", [2**63 - 1, 20], {*range(20, 37)}), ("first", [-2**63, 20], {*range(20, 37)})]
     for name, value, want_rows in cases:
         args = {"table": good_table, "lengths": good_lengths, "first": good_first, name: value}
         out_k, out_v = (torch.full((40, heads, dim), -3.0, device="cuda") for _ in range(2))
