@@ -557,15 +557,14 @@ int with_type(int type, Fn fn) {
     }
 }
 
-// calls fn with std::integral_constant of the access form; 0: the loose one
-template <int LOOSE, typename Fn>
+// calls fn with std::integral_constant of the access form; 0: the loose one.  WARP: whether kWarp is among the forms
+template <int LOOSE, bool WARP, typename Fn>
 int with_access(int a, Fn fn) {
-    switch (a) {
-        case 32: return fn(std::integral_constant<int, 32>());
-        case 16: return fn(std::integral_constant<int, 16>());
-        case kWarp: return fn(std::integral_constant<int, kWarp>());
-        default: return fn(std::integral_constant<int, LOOSE>());
-    }
+    if (a == 32) return fn(std::integral_constant<int, 32>());
+    if (a == 16) return fn(std::integral_constant<int, 16>());
+    if constexpr (WARP)
+        if (a == kWarp) return fn(std::integral_constant<int, kWarp>());
+    return fn(std::integral_constant<int, LOOSE>());
 }
 
 // calls fn with std::integral_constant of the passes: 1 or MOST

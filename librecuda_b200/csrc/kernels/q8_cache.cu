@@ -218,7 +218,7 @@ template <int LOOSE, typename T, typename Passes, typename Launch>
 int by_sides(const lcbCacheQ8 &c, const Wide &k, const Wide &v, size_t tokens, size_t rows, size_t sequences, Passes passes, Launch launch) {
     const int ka = k.access(c, rows, sizeof(T)), va = c.v_dim != 0 ? v.access(c, rows, sizeof(T)) : ka;
     auto both = [&](int access, bool with_k, bool with_v) {
-        return with_access<LOOSE>(access, [&](auto a) {
+        return with_access<LOOSE, false>(access, [&](auto a) {
             auto side = [&](const Wide &w, bool on) {
                 Side<T> s{};
                 if (!on || w.dim == 0) return s;

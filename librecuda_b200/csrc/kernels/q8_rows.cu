@@ -284,7 +284,7 @@ extern "C" int lcb_pack_q8(void *codes, void *scales, const void *src, size_t sr
             Fit fit(rows, n);
             fit.add(in);
             fit.add(out);
-            return with_access<kPackForm<T>>(fit.template access<T, true>(), [&](auto a) {
+            return with_access<kPackForm<T>, true>(fit.template access<T, true>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesPack<a()>);
                 return with_passes<kPassesPack<a()>>(s.tiling.passes, [&](auto p) {
                     return launch_rows(pack_kernel<T, a(), p()>, s, stream, out, fit.lines(in, s));
@@ -306,7 +306,7 @@ extern "C" int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void 
             Fit fit(rows, n);
             fit.add(out);
             fit.add(in);
-            return with_access<kStoreForm<T>>(fit.template access<T, false>(), [&](auto a) {
+            return with_access<kStoreForm<T>, true>(fit.template access<T, false>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesUnpack);
                 return with_passes<kPassesUnpack>(s.tiling.passes, [&](auto p) {
                     return launch_rows(unpack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), in);
@@ -333,7 +333,7 @@ extern "C" int lcb_silu_mul_pack_q8(void *h, size_t h_stride, void *gate_codes, 
             fit.add(u);
             fit.add(gp);
             fit.add(upk);
-            return with_access<kStoreForm<T>>(fit.template access<T, true>(), [&](auto a) {
+            return with_access<kStoreForm<T>, true>(fit.template access<T, true>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesSilu<a()>);
                 return with_passes<kPassesSilu<a()>>(s.tiling.passes, [&](auto p) {
                     return launch_rows(silu_mul_pack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), gp, upk, fit.lines(g, s), fit.lines(u, s));
@@ -363,7 +363,7 @@ extern "C" int lcb_silu_mul_grad_q8(void *dgate, size_t dgate_stride, void *dup,
             fit.add(d);
             fit.add(gp);
             fit.add(upk);
-            return with_access<kStoreForm<T>>(fit.template access<T, false>(), [&](auto a) {
+            return with_access<kStoreForm<T>, true>(fit.template access<T, false>(), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesGrad);
                 return launch_rows(h != nullptr ? silu_mul_grad_kernel<T, a(), true> : silu_mul_grad_kernel<T, a(), false>, s, stream,
                                    fit.lines(dg, s), fit.lines(du, s), fit.lines(out, s), fit.lines(d, s), gp, upk);
