@@ -1,7 +1,7 @@
 // The 8-bit operators as stream operations: quantising copies into and out of a paged cache, packing and unpacking of
-// matrices, and the gated unit with its 8-bit checkpoint.  A call is checked when it is recorded, with the checks of the kernel
-// layer and the stream layer's own rules for pointers, and launched by Commence like every other operation.
-// The reference has no operation that changes a number format (driverapi/include/librecuda.h:37-114).
+// matrices, and the gated unit with its 8-bit checkpoint.  A call is checked when it is recorded, with the checks of
+// the kernel layer and the stream layer's own rules for pointers, and launched by Commence like every other
+// operation. The reference has no operation that changes a number format (driverapi/include/librecuda.h:37-114).
 #include <initializer_list>
 
 #include "internal.h"
@@ -48,7 +48,8 @@ libreCudaStatus_t libreCuPackQ8(void *pCodes, void *pScales, const void *src, si
         LCU_ENSURE_CTX();
         LIBRECUDA_VALIDATE(lcb::pack_ok(pCodes, pScales, src, srcStride, type, rows, cols, false), LIBRECUDA_ERROR_INVALID_VALUE);
         if (rows == 0 || cols == 0) LIBRECUDA_SUCCEED();
-        return record_convert(stream, async, {codes(pCodes, rows, cols, true), scales(pScales, rows, cols, true), wide(src, srcStride, type, rows, cols, false)},
+        return record_convert(stream, async,
+                              {codes(pCodes, rows, cols, true), scales(pScales, rows, cols, true), wide(src, srcStride, type, rows, cols, false)},
                               [=](cudaStream_t s) { return lcb_pack_q8(pCodes, pScales, src, srcStride, type, rows, cols, s); });
     });
 }
@@ -60,7 +61,8 @@ libreCudaStatus_t libreCuUnpackQ8(void *dst, size_t dstStride, int type, const v
         LCU_ENSURE_CTX();
         LIBRECUDA_VALIDATE(lcb::pack_ok(pCodes, pScales, dst, dstStride, type, rows, cols, true), LIBRECUDA_ERROR_INVALID_VALUE);
         if (rows == 0 || cols == 0) LIBRECUDA_SUCCEED();
-        return record_convert(stream, async, {wide(dst, dstStride, type, rows, cols, true), codes(pCodes, rows, cols, false), scales(pScales, rows, cols, false)},
+        return record_convert(stream, async,
+                              {wide(dst, dstStride, type, rows, cols, true), codes(pCodes, rows, cols, false), scales(pScales, rows, cols, false)},
                               [=](cudaStream_t s) { return lcb_unpack_q8(dst, dstStride, type, pCodes, pScales, rows, cols, s); });
     });
 }

@@ -1,11 +1,11 @@
 // The 8-bit row format on the device: e4m3 codes with one power-of-two scale byte per group of 32 values.
 //
-// A group with largest finite magnitude A gets the scale s = 2^(b - 127), b the smallest of 0..246 with
-// A <= 448 s.  From the bits of A = 1.m * 2^(f - 127): 448 = 1.75 * 2^8, so s = 2^(f - 135) holds A exactly when
-// 1.m <= 1.75, i.e. m <= 0x600000, and twice that otherwise.  Adding 0x7fffff - 0x600000 to the bits carries into the
-// exponent field in just that second case, so b = ((bits + 0x1fffff) >> 23) - 8, clamped to [0, 246].  Subnormal A and
-// zero land below 0 and get b = 0, s = 2^-127.  Multiplying by 1 / s = 2^(127 - b) is exact wherever the result matters to
-// e4m3 (its smallest step is 2^-9), so the conversion to e4m3 is the only rounding.
+// A group with largest finite magnitude A gets the scale s = 2^(b - 127), b the smallest of 0..246 with A <= 448 s.
+// From the bits of A = 1.m * 2^(f - 127): 448 = 1.75 * 2^8, so s = 2^(f - 135) holds A exactly when 1.m <= 1.75, i.e.
+// m <= 0x600000, and twice that otherwise.  Adding 0x7fffff - 0x600000 to the bits carries into the exponent field in
+// just that second case, so b = ((bits + 0x1fffff) >> 23) - 8, clamped to [0, 246].  Subnormal A and zero land below
+// 0 and get b = 0, s = 2^-127.  Multiplying by 1 / s = 2^(127 - b) is exact wherever the result matters to e4m3 (its
+// smallest step is 2^-9), so the conversion to e4m3 is the only rounding.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -70,13 +70,14 @@ struct Form {
 };
 
 // ---- which units a lane works on --------------------------------------------------------------------------------
-// The data is `lines` lines (rows of a matrix, tokens of a cache) of `width` units each, a row padded to whole groups.  A
-// CTA takes `passes` units per lane, at the same place of as many lines, so a lane knows its column once and only steps its
-// pointers from line to line.  Lines of up to kMaxThreads units: several lie side by side in a CTA.  Longer ones: `chunks`
-// CTAs share a line in even parts.  Parts start at multiples of 32 lanes, lines at multiples of a group's lanes, so
-// the lanes of a group are neighbours in one warp.  A grid that would not fill half of the GPU that way takes one
-// pass (pack 3000x4096 bf16: 5.7 us with the border at half of the resident CTAs, 7.1 at all of them; 1000x4096: 2.3, and 2.7 at a
-// sixteenth).  128 threads: with 256 the gated unit takes 113 us instead of 101, a cache write 64 instead of 61.
+// The data is `lines` lines (rows of a matrix, tokens of a cache) of `width` units each, a row padded to whole
+// groups.  A CTA takes `passes` units per lane, at the same place of as many lines, so a lane knows its column once
+// and only steps its pointers from line to line.  Lines of up to kMaxThreads units: several lie side by side in a
+// CTA.  Longer ones: `chunks` CTAs share a line in even parts.  Parts start at multiples of 32 lanes, lines at
+// multiples of a group's lanes, so the lanes of a group are neighbours in one warp.  A grid that would not fill half
+// of the GPU that way takes one pass (pack 3000x4096 bf16: 5.7 us with the border at half of the resident CTAs, 7.1
+// at all of them; 1000x4096: 2.3, and 2.7 at a sixteenth).  128 threads: with 256 the gated unit takes 113 us instead
+// of 101, a cache write 64 instead of 61.
 constexpr int kMaxThreads = 128;
 struct Tiling {
     uint64_t width, lines;
@@ -125,9 +126,9 @@ struct Lane {
 };
 
 // ---- a warp's run of values -----------------------------------------------------------------------------------------
-// Up to 512 values of T that lie behind each other at any address, 16 to a lane, accessed in aligned words, lane by lane side by
-// side.  In shared memory a lane's words have one word of room behind them, so that the accesses by word and those by lane
-// both find 32 different banks.
+// Up to 512 values of T that lie behind each other at any address, 16 to a lane, accessed in aligned words, lane by
+// lane side by side.  In shared memory a lane's words have one word of room behind them, so that the accesses by word
+// and those by lane both find 32 different banks.
 template <typename T>
 struct Run {
     static constexpr int kLaneWords = 16 * (int)sizeof(T) / 4;
@@ -266,8 +267,8 @@ struct Unit {  // as it lies in memory
 #pragma unroll
         for (int i = 0; i < kWords; ++i) w[i] = 0;
     }
-    // `left`: columns from the unit's first one to the end of the row, 0: no unit.  Values behind the end are 0.  Every lane
-    // of the warp calls this, take() before it looks at a value, and store().
+    // `left`: columns from the unit's first one to the end of the row, 0: no unit.  Values behind the end are 0.
+    // Every lane of the warp calls this, take() before it looks at a value, and store().
     __device__ __forceinline__ void load(const T *p, int left) {
         const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
         clear();
@@ -280,7 +281,8 @@ struct Unit {  // as it lies in memory
 #pragma unroll
             for (int i = 0; i < kWords; i += 8)
                 asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
+                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]),
+                               "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
                              : "l"(q + i));
         } else if constexpr (A == 16) {  // the lanes' accesses interleave: the second one finds its sectors in L1
 #pragma unroll
@@ -292,7 +294,8 @@ struct Unit {  // as it lies in memory
 #pragma unroll
             for (int i = 0; i < kWords; ++i) w[i] = i < left ? q[i] : 0u;
         } else {
-            // the aligned words that hold at least one of the values, shifted by half a word where the address asks for it
+            // the aligned words that hold at least one of the values, shifted by half a word where the address asks
+            // for it
             const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(p) >> 1) & 1u;
             q = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
             const int n = min(left, kValues) + (int)odd;
@@ -329,7 +332,8 @@ struct Unit {  // as it lies in memory
 #pragma unroll
             for (int i = 0; i < kWords; i += 8)
                 asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                             :: "l"(q + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                             :: "l"(q + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
+                                "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
                              : "memory");
         } else if constexpr (A == 16) {
 #pragma unroll
@@ -481,7 +485,8 @@ struct Codes {  // of one unit, four to a word
             }
         }
     }
-    // values j and j + 1 (j even), in 32 bits: a code is an f16 value exactly, and its product with a power of two is exact
+    // values j and j + 1 (j even), in 32 bits: a code is an f16 value exactly, and its product with a power of two is
+    // exact
     __device__ __forceinline__ Pair pair(int j, Pair scale) const {
         uint32_t r;
         asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)(w[j / 4] >> (8 * (j & 2)))));
@@ -490,9 +495,9 @@ struct Codes {  // of one unit, four to a word
     }
 };
 
-// Packs a unit; returns the scale byte of its group.  Every lane of the warp calls it; lanes without values come with a
-// cleared unit.  The maximum ignores NaN, which convert to the NaN code by themselves; infinities are rare, so only when one
-// is found somewhere in the warp the values are looked at one by one.
+// Packs a unit; returns the scale byte of its group.  Every lane of the warp calls it; lanes without values come with
+// a cleared unit.  The maximum ignores NaN, which convert to the NaN code by themselves; infinities are rare, so only
+// when one is found somewhere in the warp the values are looked at one by one.
 template <typename T, int A>
 __device__ __forceinline__ unsigned pack_unit(const Unit<T, A> &in, Codes<A> &out) {
     constexpr int N = Form<A>::kValues;
@@ -521,11 +526,10 @@ __device__ __forceinline__ unsigned pack_unit(const Unit<T, A> &in, Codes<A> &ou
 }
 
 // ---- sigmoid --------------------------------------------------------------------------------------------------
-// s = 1 / (1 + e) and q = 1 - s = e * s with e = exp(-g): no term cancels, so both are good to a few roundings wherever they
-// are normal numbers.  g is held to [-88, 100]: below, s is subnormal and becomes 0; above, e does.  e is finite for all of
-// them, and an infinite or NaN g still shows in g * s.
-// e = 2^t * (1 - ln2 * rest) with t = -g log2(e) rounded and rest what the rounding left of g log2(e), since an error of t
-// counts |t| times.
+// s = 1 / (1 + e) and q = 1 - s = e * s with e = exp(-g): no term cancels, so both are good to a few roundings
+// wherever they are normal numbers.  g is held to [-88, 100]: below, s is subnormal and becomes 0; above, e does.  e
+// is finite for all of them, and an infinite or NaN g still shows in g * s. e = 2^t * (1 - ln2 * rest) with t = -g
+// log2(e) rounded and rest what the rounding left of g log2(e), since an error of t counts |t| times.
 struct Sigmoid {
     Pair s, q;
 };

@@ -1,17 +1,19 @@
 // Paged key/value cache in the 8-bit row format for sm_100a: quantising rows as they are written to their slots, and
 // reading sequences back through a page table.
 //
-// Units, groups and rounding are those of q8.cuh; a row is a token's head, a line a token with all its heads, so that a lane keeps
-// its place in the heads and steps from token to token.  Keys and values share a launch.  Every index that comes from device memory
-// (slots, pages, lengths, first rows) is checked before it forms an address.
+// Units, groups and rounding are those of q8.cuh; a row is a token's head, a line a token with all its heads, so that
+// a lane keeps its place in the heads and steps from token to token.  Keys and values share a launch.  Every index
+// that comes from device memory (slots, pages, lengths, first rows) is checked before it forms an address.
 //
-// What bounds them: HBM, 3.03 bytes per value of bf16, and for a read the chain length -> page -> code in front of it.  A CTA of
-// 128 threads holds few tokens, so the chain is walked by many CTAs at once; a write loads its rows beside their slots.
+// What bounds them: HBM, 3.03 bytes per value of bf16, and for a read the chain length -> page -> code in front of
+// it.  A CTA of 128 threads holds few tokens, so the chain is walked by many CTAs at once; a write loads its rows
+// beside their slots.
 //
-// Measured on a B200 (bf16, 8 heads of 128; share of 6548 GB/s): write of 65000 tokens, a sixteenth of them padding, 61 us, 95 % (65 us
-// and 89 % heads first: 128-byte pieces); read of 48 sequences of 1 to 16384 tokens 377 us, 99 %; in f32 100 %.  Heads of 65: 83 us
-// and 36 %, 517 us and 37 %, rows at any address that are too short for a warp.  One token: write 1.05 us in a graph.
-// One lane per value instead of 16: 997 and 9805 us.  Rows loaded only once their slots are known: 65 us against 61.
+// Measured on a B200 (bf16, 8 heads of 128; share of 6548 GB/s): write of 65000 tokens, a sixteenth of them padding,
+// 61 us, 95 % (65 us and 89 % heads first: 128-byte pieces); read of 48 sequences of 1 to 16384 tokens 377 us, 99 %;
+// in f32 100 %.  Heads of 65: 83 us and 36 %, 517 us and 37 %, rows at any address that are too short for a warp.
+// One token: write 1.05 us in a graph. One lane per value instead of 16: 997 and 9805 us.  Rows loaded only once
+// their slots are known: 65 us against 61.
 #include <algorithm>
 
 #include "lcb200_kernels.h"
@@ -21,11 +23,13 @@
 namespace lcb {
 namespace {
 
-// Tokens in flight per lane, where there is work for that many.  Write: 4 (61 us; 2: 65; 1: 76).  Read: 2 (377 us; 4: 378; 1: 422).
+// Tokens in flight per lane, where there is work for that many.  Write: 4 (61 us; 2: 65; 1: 76).  Read: 2 (377 us; 4:
+// 378; 1: 422).
 template <int A>
 constexpr int kPassesWrite = A >= 16 ? 4 : 2;
 constexpr int kPassesRead = 2;
-// Heads at any address: values per lane of a write (65 columns: bf16 84 us with 16, f32 48 with 8, 52 with 16); a read takes 8.
+// Heads at any address: values per lane of a write (65 columns: bf16 84 us with 16, f32 48 with 8, 52 with 16); a
+// read takes 8.
 template <typename T>
 constexpr int kWriteForm = sizeof(T) == 4 ? kLooseShort : kLoose;
 constexpr int kRunTiles = 4, kRunWaves = 4, kMostWaves = 64;  // tiles that a CTA of a read takes, see its launcher
@@ -89,8 +93,8 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
     Unit<T, A> x[P];
     int64_t slot[P];
     pdl_wait();
-    // The rows of skipped tokens are loaded too: waiting for the slot first would put a second memory latency in front of
-    // every row.
+    // The rows of skipped tokens are loaded too: waiting for the slot first would put a second memory latency in
+    // front of every row.
 #pragma unroll
     for (int u = 0; u < P; ++u) {
         const uint64_t token = at.token + u * at.step;
@@ -131,9 +135,9 @@ struct Sequences {
     FastDiv32 blocks;  // of one sequence, keys and values
 };
 
-// A CTA takes `tiles` tiles of one sequence, one behind the other: in a ragged batch much of the grid lies behind the ends
-// of the sequences, and a CTA that finds nothing to do costs a launch and a memory latency all the same (377 us with up to 4
-// tiles, 404 with one, 384 with 8, which leave too few CTAs to even out the sequences).
+// A CTA takes `tiles` tiles of one sequence, one behind the other: in a ragged batch much of the grid lies behind the
+// ends of the sequences, and a CTA that finds nothing to do costs a launch and a memory latency all the same (377 us
+// with up to 4 tiles, 404 with one, 384 with 8, which leave too few CTAs to even out the sequences).
 template <typename T, int A, int P>
 __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side<T> v, Pool pool, Sequences q, ErrorSink errors) {
     pdl_launch_dependents();
@@ -215,7 +219,8 @@ struct Wide {  // the wide tensor of a side, as given
 // Keys and values go to one launch where their accesses are the same, else to one each.
 // launch(access, passes, k side, v side): either side may have no blocks.  passes(access): at most.
 template <int LOOSE, typename T, typename Passes, typename Launch>
-int by_sides(const lcbCacheQ8 &c, const Wide &k, const Wide &v, size_t tokens, size_t rows, size_t sequences, Passes passes, Launch launch) {
+int by_sides(const lcbCacheQ8 &c, const Wide &k, const Wide &v, size_t tokens, size_t rows, size_t sequences, Passes passes,
+             Launch launch) {
     const int ka = k.access(c, rows, sizeof(T)), va = c.v_dim != 0 ? v.access(c, rows, sizeof(T)) : ka;
     auto both = [&](int access, bool with_k, bool with_v) {
         return with_access<LOOSE, false>(access, [&](auto a) {
@@ -273,12 +278,14 @@ extern "C" int lcb_cache_write_q8(const lcbCacheQ8 *cache, const void *k, size_t
     const Wide vw{v, v_token_stride, v_head_stride, cache->v_dim, cache->v_codes, cache->v_scales};
     return with_type(type, [&](auto *t) {
         using T = const std::remove_pointer_t<decltype(t)>;
-        return by_sides<kWriteForm<T>, T>(*cache, kw, vw, tokens, tokens, 1, [](auto a) { return kPassesWrite<decltype(a)::value>; }, [&](auto a, auto p, const Side<T> &ks, const Side<T> &vs) {
+        auto passes = [](auto a) { return kPassesWrite<decltype(a)::value>; };
+        return by_sides<kWriteForm<T>, T>(*cache, kw, vw, tokens, tokens, 1, passes,
+                                          [&](auto a, auto p, const Side<T> &ks, const Side<T> &vs) {
             const uint64_t blocks = (uint64_t)ks.blocks + vs.blocks;
             if (blocks > 0x7fffffffu) return 1;
             const unsigned threads = std::max(ks.tiling.threads, vs.tiling.threads);
-            return launch_kernel(cache_write_kernel<std::remove_const_t<T>, a(), p()>, (unsigned)blocks, threads, 0, static_cast<cudaStream_t>(stream),
-                                 ks, vs, pool_of(*cache), slots, (uint64_t)tokens, errors);
+            return launch_kernel(cache_write_kernel<std::remove_const_t<T>, a(), p()>, (unsigned)blocks, threads, 0,
+                                 static_cast<cudaStream_t>(stream), ks, vs, pool_of(*cache), slots, (uint64_t)tokens, errors);
         });
     });
 }
@@ -297,9 +304,11 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
     const Wide vw{v, v_token_stride, v_head_stride, cache->v_dim, cache->v_codes, cache->v_scales};
     return with_type(type, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return by_sides<kLooseShort, T>(*cache, kw, vw, max_length, rows, sequences, [](auto) { return kPassesRead; }, [&](auto a, auto p, const Side<T> &ks, const Side<T> &vs) {
-            // Up to kRunTiles tiles to a CTA while that leaves the GPU kRunWaves grids of resident CTAs, and more of them
-            // where the grid would have more than kMostWaves: max_length may be far above the lengths.
+        auto passes = [](auto) { return kPassesRead; };
+        return by_sides<kLooseShort, T>(*cache, kw, vw, max_length, rows, sequences, passes,
+                                        [&](auto a, auto p, const Side<T> &ks, const Side<T> &vs) {
+            // Up to kRunTiles tiles to a CTA while that leaves the GPU kRunWaves grids of resident CTAs, and more of
+            // them where the grid would have more than kMostWaves: max_length may be far above the lengths.
             const uint64_t all = ((uint64_t)ks.blocks + vs.blocks) * sequences, wave = Tiling::resident_ctas();
             const uint32_t tiles = (uint32_t)std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(all / (wave * kRunWaves), 1), kRunTiles),
                                                                 std::min<uint64_t>(all / (wave * kMostWaves), 0x7fffffffu));
@@ -315,8 +324,8 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
             if (ks.blocks > 0x7fffffffu || vs.blocks > 0x7fffffffu || each > 0x7fffffffu || sequences > 0x7fffffffu / each) return 1;
             const Sequences q{page_table, lengths, first_rows, table_stride, rows, (uint32_t)max_length, tiles, FastDiv32::of((uint32_t)each)};
             const unsigned threads = std::max(ks.tiling.threads, vs.tiling.threads);
-            return launch_kernel(cache_read_kernel<T, a(), p()>, (unsigned)(each * sequences), threads, 0, static_cast<cudaStream_t>(stream), kr, vr,
-                                 pool_of(*cache), q, errors);
+            return launch_kernel(cache_read_kernel<T, a(), p()>, (unsigned)(each * sequences), threads, 0,
+                                 static_cast<cudaStream_t>(stream), kr, vr, pool_of(*cache), q, errors);
         });
     });
 }

@@ -43,7 +43,8 @@ inline bool rows_apart(size_t rows, size_t stride, size_t cols) { return rows <=
 inline bool heads_apart(size_t tokens, size_t token_stride, size_t heads, size_t head_stride, size_t dim) {
     if (tokens <= 1) return rows_apart(heads, head_stride, dim);
     if (heads <= 1) return rows_apart(tokens, token_stride, dim);
-    const size_t across_heads = span_bytes(1, 0, heads, head_stride, dim, 1), across_tokens = span_bytes(1, 0, tokens, token_stride, dim, 1);
+    const size_t across_heads = span_bytes(1, 0, heads, head_stride, dim, 1);
+    const size_t across_tokens = span_bytes(1, 0, tokens, token_stride, dim, 1);
     return (head_stride >= dim && across_heads != 0 && token_stride >= across_heads) ||
            (token_stride >= dim && across_tokens != 0 && head_stride >= across_tokens);
 }
@@ -59,7 +60,8 @@ inline bool packed_matrix_ok(const void *codes, const void *scales, size_t rows,
 inline bool pack_ok(const void *codes, const void *scales, const void *wide, size_t stride, int type, size_t rows, size_t cols, bool wide_is_output) {
     if (!type_ok(type)) return false;
     if (rows == 0 || cols == 0) return true;
-    return codes != scales && codes != wide && scales != wide && packed_matrix_ok(codes, scales, rows, cols) && wide_matrix_ok(wide, stride, type, rows, cols, wide_is_output);
+    return codes != scales && codes != wide && scales != wide && packed_matrix_ok(codes, scales, rows, cols) &&
+           wide_matrix_ok(wide, stride, type, rows, cols, wide_is_output);
 }
 
 inline bool silu_pack_ok(const void *h, size_t h_stride, const void *gate_codes, const void *gate_scales, const void *up_codes, const void *up_scales,
@@ -67,7 +69,8 @@ inline bool silu_pack_ok(const void *h, size_t h_stride, const void *gate_codes,
     if (!type_ok(type)) return false;
     if (rows == 0 || cols == 0) return true;
     return apart({h, gate_codes, gate_scales, up_codes, up_scales}) && packed_matrix_ok(gate_codes, gate_scales, rows, cols) &&
-           packed_matrix_ok(up_codes, up_scales, rows, cols) && wide_matrix_ok(h, h_stride, type, rows, cols, true) && wide_matrix_ok(gate, gate_stride, type, rows, cols, false) &&
+           packed_matrix_ok(up_codes, up_scales, rows, cols) && wide_matrix_ok(h, h_stride, type, rows, cols, true) &&
+           wide_matrix_ok(gate, gate_stride, type, rows, cols, false) &&
            wide_matrix_ok(up, up_stride, type, rows, cols, false);
 }
 inline bool silu_grad_ok(const void *dgate, size_t dgate_stride, const void *dup, size_t dup_stride, const void *h, size_t h_stride, const void *dh,
@@ -114,7 +117,8 @@ inline bool cache_write_ok(const lcbCacheQ8 *c, const void *k, size_t kts, size_
                            const int64_t *slots, size_t tokens) {
     if (!cache_ok(c) || !type_ok(type)) return false;
     if (tokens == 0) return true;
-    return apart({c->k_codes, c->k_scales, c->v_codes, c->v_scales}) && slots != nullptr && aligned(slots, 8) && cache_rows_ok(*c, k, kts, khs, v, vts, vhs, type, tokens, false);
+    return apart({c->k_codes, c->k_scales, c->v_codes, c->v_scales}) && slots != nullptr && aligned(slots, 8) &&
+           cache_rows_ok(*c, k, kts, khs, v, vts, vhs, type, tokens, false);
 }
 inline bool cache_read_ok(const lcbCacheQ8 *c, const void *k, size_t kts, size_t khs, const void *v, size_t vts, size_t vhs, int type,
                           const int32_t *table, size_t table_stride, const int32_t *lengths, const int64_t *first_rows, size_t sequences,

@@ -1,22 +1,24 @@
-// 8-bit activation checkpoints for sm_100a: packing and unpacking a matrix, and the gated unit gate * up / (1 + exp(-gate))
-// that leaves its checkpoint in the forward pass and reads it in the backward pass.
+// 8-bit activation checkpoints for sm_100a: packing and unpacking a matrix, and the gated unit gate * up / (1 +
+// exp(-gate)) that leaves its checkpoint in the forward pass and reads it in the backward pass.
 //
-// What they compute (format and rounding: q8.cuh).  pack: codes and scales of every group.  unpack: code * s, rounded once.
-// silu_mul_pack: h = g u s(g) with s(g) = 1 / (1 + exp(-g)), and g and u packed.  silu_mul_grad, with g and u the values of
-// the packed pair: dup = dh g s(g), dgate = dh u s(g) (1 + g (1 - s(g))), and h again.
+// What they compute (format and rounding: q8.cuh).  pack: codes and scales of every group.  unpack: code * s, rounded
+// once. silu_mul_pack: h = g u s(g) with s(g) = 1 / (1 + exp(-g)), and g and u packed.  silu_mul_grad, with g and u
+// the values of the packed pair: dup = dh g s(g), dgate = dh u s(g) (1 + g (1 - s(g))), and h again.
 //
-// What bounds them: HBM.  Every byte is moved once; per value of bf16 that is 3.03 bytes for pack and unpack, 8.06 for the gated
-// unit, 8.06 for its gradient, 10.06 with h again.  The arithmetic (about 7, 25 and 25 instructions per value, shared addresses
-// counted) is the next limit, at 45-65 % of the issue slots, and what any form that spends more per value runs into first.  So a
-// lane holds 16 values, 32-bit arithmetic goes two to an instruction, magnitudes are compared before they are converted, addresses
-// are found once per lane, and all loads of a CTA are issued before its first store.  No tensor cores: there is no product.
+// What bounds them: HBM.  Every byte is moved once; per value of bf16 that is 3.03 bytes for pack and unpack, 8.06
+// for the gated unit, 8.06 for its gradient, 10.06 with h again.  The arithmetic (about 7, 25 and 25 instructions per
+// value, shared addresses counted) is the next limit, at 45-65 % of the issue slots, and what any form that spends
+// more per value runs into first.  So a lane holds 16 values, 32-bit arithmetic goes two to an instruction,
+// magnitudes are compared before they are converted, addresses are found once per lane, and all loads of a CTA are
+// issued before its first store.  No tensor cores: there is no product.
 //
-// Measured on a B200 (bf16 unless said; share of 6548 GB/s, what a copy of the same bytes by torch reaches): pack 16384 x 8192
-// 59 us, 105 %; unpack 61 us, 102 %; unpack 16400 x 5120 to f32 63.6 us, 101 %; gated unit 8192 x 10240 101 us, 102 %; its gradient
-// with h again 125.5 us, 103 %, without 101 us.  Rows of 16-byte alignment: pack 16384 x 8200 69 us, 91 %.  Rows at any
-// address: pack 16384 x 8191 102 us, unpack 86 us, gated unit 8192 x 10241 195 us, gradient 172 us: 53-72 %, bound by issue slots and
-// L1 accesses; f32 with 1001 columns: pack 32, unpack 29 of 23 us.  Smallest calls: 1.1-1.6 us in a graph.
-// One lane per value instead of 16: pack 542 us, unpack to f32 339, gated unit 503, gradient 405.
+// Measured on a B200 (bf16 unless said; share of 6548 GB/s, what a copy of the same bytes by torch reaches): pack
+// 16384 x 8192 59 us, 105 %; unpack 61 us, 102 %; unpack 16400 x 5120 to f32 63.6 us, 101 %; gated unit 8192 x 10240
+// 101 us, 102 %; its gradient with h again 125.5 us, 103 %, without 101 us.  Rows of 16-byte alignment: pack 16384 x
+// 8200 69 us, 91 %.  Rows at any address: pack 16384 x 8191 102 us, unpack 86 us, gated unit 8192 x 10241 195 us,
+// gradient 172 us: 53-72 %, bound by issue slots and L1 accesses; f32 with 1001 columns: pack 32, unpack 29 of 23
+// us.  Smallest calls: 1.1-1.6 us in a graph. One lane per value instead of 16: pack 542 us, unpack to f32 339, gated
+// unit 503, gradient 405.
 #include "lcb200_kernels.h"
 #include "q8.cuh"
 #include "q8_check.h"
@@ -24,23 +26,25 @@
 namespace lcb {
 namespace {
 
-// Units in flight per lane, where there is work for that many.  Pack: 4 (59.1 us; 3 and 2 within 1 %, 1: 64).  Unpack: 2 (60.9 us;
-// 1: 69).  Gated unit: 2 of each input (101 us; 1: 106); in the warp form 1 (201 us; 2: 236, whose loads no longer fit
-// L1).  Gradient: 1, which already has three inputs in flight and three outputs to hold; 2 take 86 registers and 169 us against 125.
+// Units in flight per lane, where there is work for that many.  Pack: 4 (59.1 us; 3 and 2 within 1 %, 1: 64).
+// Unpack: 2 (60.9 us; 1: 69).  Gated unit: 2 of each input (101 us; 1: 106); in the warp form 1 (201 us; 2: 236,
+// whose loads no longer fit L1).  Gradient: 1, which already has three inputs in flight and three outputs to hold; 2
+// take 86 registers and 169 us against 125.
 template <int A>
 constexpr int kPassesPack = A >= 16 ? 4 : 2;
 constexpr int kPassesUnpack = 2;
 template <int A>
 constexpr int kPassesSilu = A == kWarp ? 1 : 2;
 constexpr int kPassesGrad = 1;
-// Rows at any address give each row warps of its own from here on.  Below, lanes behind the end of a row cost more than the
-// side-by-side accesses save.  16-bit types: 333 columns of bf16 take 104 us against 82 in the gated unit, 500 columns 66 against
-// 68.  f32 with packing: 333 columns 44 us against 40 to pack, 500 columns 30 against 37; without: 259 columns 41 us against 60 to
-// unpack, 200 columns equal.
+// Rows at any address give each row warps of its own from here on.  Below, lanes behind the end of a row cost more
+// than the side-by-side accesses save.  16-bit types: 333 columns of bf16 take 104 us against 82 in the gated unit,
+// 500 columns 66 against 68.  f32 with packing: 333 columns 44 us against 40 to pack, 500 columns 30 against 37;
+// without: 259 columns 41 us against 60 to unpack, 200 columns equal.
 template <typename T, bool PACKS>
 constexpr size_t kWarpColumns = sizeof(T) == 2 ? 448 : PACKS ? 400 : 224;
-// Rows that stay below: values per lane.  Loads of 32-bit values share sectors less, so fewer to a lane; stores still fewer (100
-// columns of f32: pack 35 us with 8, 45 with 16, 40 with 4; unpack 48 with 4, 74 with 8; the 16-bit types the other way round).
+// Rows that stay below: values per lane.  Loads of 32-bit values share sectors less, so fewer to a lane; stores still
+// fewer (100 columns of f32: pack 35 us with 8, 45 with 16, 40 with 4; unpack 48 with 4, 74 with 8; the 16-bit types
+// the other way round).
 template <typename T>
 constexpr int kPackForm = sizeof(T) == 4 ? kLooseShort : kLoose;
 template <typename T>
@@ -55,8 +59,8 @@ struct Packed {
     uint8_t *codes, *scales;
 };
 
-// A matrix whose rows lie behind each other without a gap and end with whole groups is one long row, and so is a single row.  It
-// is cut into lines of kMaxThreads units, which keeps every lane busy whatever the number of columns.
+// A matrix whose rows lie behind each other without a gap and end with whole groups is one long row, and so is a
+// single row.  It is cut into lines of kMaxThreads units, which keeps every lane busy whatever the number of columns.
 struct Shape {
     uint64_t rows, cols, groups;
     uint64_t flat;  // values of one long row, else 0
@@ -218,8 +222,8 @@ __global__ void __launch_bounds__(kMaxThreads) silu_mul_grad_kernel(Rows<T> dgat
     if constexpr (AGAIN) y.store(at.wide(h), left, scratch);
 }
 
-// The widest accesses that are aligned in every row.  A row's codes lie behind each other, so the columns must be a multiple of
-// what an access covers.
+// The widest accesses that are aligned in every row.  A row's codes lie behind each other, so the columns must be a
+// multiple of what an access covers.
 struct Fit {
     size_t rows, cols;
     bool flat;
