@@ -27,12 +27,13 @@ namespace lcb {
 namespace {
 
 // Units in flight per lane, where there is work for that many.  Pack: 4 (59.1 us; 3 and 2 within 1 %, 1: 64).
-// Unpack: 2 (60.9 us; 1: 69).  Gated unit: 2 of each input (101 us; 1: 106); in the warp form 1 (201 us; 2: 236,
-// whose loads no longer fit L1).  Gradient: 1, which already has three inputs in flight and three outputs to hold; 2
-// take 86 registers and 169 us against 125.
+// Unpack: 2 (60.9 us; 1: 69), in the warp form 1 (84.7 us at 16384 x 8191; 2: 86.9).  Gated unit: 2 of each input (101
+// us; 1: 106), in the warp form 1 (201 us; 2: 236, whose loads no longer fit L1).  Gradient: 1, which already has three
+// inputs in flight and three outputs to hold; 2 take 86 registers and 169 us against 125.
 template <int A>
 constexpr int kPassesPack = A >= 16 ? 4 : 2;
-constexpr int kPassesUnpack = 2;
+template <int A>
+constexpr int kPassesUnpack = A == kWarp ? 1 : 2;
 template <int A>
 constexpr int kPassesSilu = A == kWarp ? 1 : 2;
 constexpr int kPassesGrad = 1;
@@ -311,8 +312,8 @@ extern "C" int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void 
             fit.add(out);
             fit.add(in);
             return with_access<kStoreForm<T>, true>(fit.template access<T, false>(), [&](auto a) {
-                const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesUnpack);
-                return with_passes<kPassesUnpack>(s.tiling.passes, [&](auto p) {
+                const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesUnpack<a()>);
+                return with_passes<kPassesUnpack<a()>>(s.tiling.passes, [&](auto p) {
                     return launch_rows(unpack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), in);
                 });
             });
