@@ -136,7 +136,9 @@ int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void *codes, con
                   lcbStream stream);
 
 /* The gated unit h = gate * up / (1 + exp(-gate)) that leaves its checkpoint in the same pass: `gate` and `up` packed as
- * lcb_pack_q8 packs them.  h is computed from the wide inputs in 32 bits and rounded once. */
+ * lcb_pack_q8 packs them.  h is computed from the wide inputs in 32 bits and rounded once.  In 32 bits exp(-gate) is infinite
+ * below gate = -88.72, so the sigmoid is 0 there; between that and -87.34 it is a subnormal number, held in steps of 2^-149. The
+ * same holds for the backward pass. */
 int lcb_silu_mul_pack_q8(void *h, size_t h_stride, void *gate_codes, void *gate_scales, void *up_codes, void *up_scales, const void *gate,
                          size_t gate_stride, const void *up, size_t up_stride, int type, size_t rows, size_t cols, lcbStream stream);
 /* Its backward pass from the checkpoint: with g, u the values of the packed gate and up, s = 1 / (1 + exp(-g)) and dh

@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kMaxThreads, A == kWarp ? 6 : 0) silu_mul_pack
 #pragma unroll
             for (int j = 0; j < Form<A>::kValues; j += 2) {
                 const Pair x = g[k].pair(j);
-                out.template set_pair<false>(j, x * sigmoid(x).s * u[k].pair(j));
+                out.template set_pair<false>(j, x * sigmoid<false>(x).s * u[k].pair(j));
             }
             out.store(to + k * (at.step * h.stride), at.columns(k), scratch);
         }
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kMaxThreads) silu_mul_grad_kernel(Rows<T> dgat
 #pragma unroll
     for (int j = 0; j < Form<A>::kValues; j += 2) {
         const Pair x = g.pair(j, gs), z = u.pair(j, us), dj = d.pair(j);
-        const Sigmoid sg = sigmoid(x);
+        const Sigmoid sg = sigmoid<true>(x);
         const Pair silu = x * sg.s;
         du.template set_pair<false>(j, dj * silu);
         dg.template set_pair<false>(j, dj * z * fma2(silu, sg.q, sg.s));
