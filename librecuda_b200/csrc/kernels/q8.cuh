@@ -15,41 +15,13 @@
 
 #include "common.cuh"
 #include "lcb200_types.h"
+#include "q8_tiling.h"
 
 namespace lcb {
 
 constexpr int kGroup = 32;          // values per scale byte
 constexpr int kMaxScaleByte = 246;  // 448 * 2^(246 - 127) is finite in f32 and bf16, so no value of a code overflows
 constexpr unsigned kInfBits = 0x7f800000u;
-
-// ---- division by a launch constant ----------------------------------------------------------------------------
-// magic = floor((2^bits - 1) / d): the high half of n * magic is the quotient or one less, for every n of `bits` bits.
-struct FastDiv {
-    uint64_t magic, d;
-    static FastDiv of(uint64_t d) { return {~0ull / d, d}; }
-    __device__ __forceinline__ uint64_t divmod(uint64_t n, uint64_t &rest) const {
-        uint64_t q = __umul64hi(n, magic);
-        rest = n - q * d;
-        if (rest >= d) {
-            rest -= d;
-            ++q;
-        }
-        return q;
-    }
-};
-struct FastDiv32 {
-    uint32_t magic, d;
-    static FastDiv32 of(uint32_t d) { return {~0u / d, d}; }
-    __device__ __forceinline__ uint32_t divmod(uint32_t n, uint32_t &rest) const {
-        uint32_t q = __umulhi(n, magic);
-        rest = n - q * d;
-        if (rest >= d) {
-            rest -= d;
-            ++q;
-        }
-        return q;
-    }
-};
 
 // ---- units --------------------------------------------------------------------------------------------------------
 // A unit is kValues consecutive values of a row, held by one lane; kLanes neighbouring lanes hold a group.  Its accesses come
