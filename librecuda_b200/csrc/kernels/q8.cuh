@@ -19,64 +19,10 @@
 
 namespace lcb {
 
-constexpr int kGroup = 32;          // values per scale byte
 constexpr int kMaxScaleByte = 246;  // 448 * 2^(246 - 127) is finite in f32 and bf16, so no value of a code overflows
 constexpr unsigned kInfBits = 0x7f800000u;
 
-// ---- units --------------------------------------------------------------------------------------------------------
-// A unit is kValues consecutive values of a row, held by one lane; kLanes neighbouring lanes hold a group.  Its accesses come
-// in forms A.
-//   32, 16        bytes of an access to the wide type (the codes then in 16 or 8 bytes); a row ends with a whole unit, or with
-//                 8 or 16 values of one
-//   kWarp         rows at any address, ending anywhere, a warp inside one row: as kLoose, but the warp loads and stores its 512
-//                 wide values as a run of words side by side, handed over through shared memory
-//   kLoose, kLooseShort, kLooseTiny
-//                 rows at any address too short to give a warp to each: a lane fetches its 16, 8 or 4 values in the words that
-//                 the address allows.  A warp then touches many sectors at once; loads find them again in L1, stores do
-//                 not, so what a kernel moves decides how many values serve it best.
-constexpr int kWarp = 1, kLooseShort = 2, kLooseTiny = 3, kLoose = 4;
-template <int A>
-struct Form {
-    static constexpr int kValues = A == kLooseTiny ? 4 : A == kLooseShort ? 8 : 16;
-    static constexpr int kLanes = kGroup / kValues;
-};
-
-// ---- which units a lane works on --------------------------------------------------------------------------------
-// The data is `lines` lines (rows of a matrix, tokens of a cache) of `width` units each, a row padded to whole
-// groups.  A CTA takes `passes` units per lane, at the same place of as many lines, so a lane knows its column once
-// and only steps its pointers from line to line.  Lines of up to kMaxThreads units: several lie side by side in a
-// CTA.  Longer ones: `chunks` CTAs share a line in even parts.  Parts start at multiples of 32 lanes, lines at
-// multiples of a group's lanes, so the lanes of a group are neighbours in one warp.  A grid that would not fill half
-// of the GPU that way takes one pass (pack 3000x4096 bf16: 5.7 us with the border at half of the resident CTAs, 7.1
-// at all of them; 1000x4096: 2.3, and 2.7 at a sixteenth).  128 threads: with 256 the gated unit takes 113 us instead
-// of 101, a cache write 64 instead of 61.
-constexpr int kMaxThreads = 128;
-struct Tiling {
-    uint64_t width, lines;
-    FastDiv32 by_chunks, by_width;  // by_width: of lines that lie side by side, else 0 / 1
-    uint32_t threads, side_by_side, passes;
-    // `times`: how often the launch repeats the tiling
-    static Tiling of(uint64_t lines, uint64_t width, uint32_t passes, uint64_t times = 1) {
-        Tiling t{width, lines, FastDiv32::of(1), FastDiv32::of(1), 0, 1, passes};
-        if (width <= kMaxThreads) {
-            t.by_width = FastDiv32::of((uint32_t)width);
-            t.side_by_side = (uint32_t)(kMaxThreads / width);
-            if (t.side_by_side > lines) t.side_by_side = (uint32_t)lines;
-            t.threads = (uint32_t)((t.side_by_side * width + 31) / 32 * 32);
-        } else {
-            const uint64_t chunks = (width + kMaxThreads - 1) / kMaxThreads;
-            t.by_chunks = FastDiv32::of((uint32_t)chunks);
-            t.threads = (uint32_t)(((width + chunks - 1) / chunks + 31) / 32 * 32);
-        }
-        if (t.blocks() * times < resident_ctas() / 2) t.passes = 1;
-        return t;
-    }
-    static uint64_t resident_ctas() { return (uint64_t)sm_count() * (2048 / kMaxThreads); }
-    uint64_t blocks() const {
-        const uint64_t tile = (uint64_t)side_by_side * passes;
-        return (lines + tile - 1) / tile * by_chunks.d;
-    }
-};
+// ---- a lane's place (tilings: q8_tiling.h) ------------------------------------------------------------------------
 struct Lane {
     uint64_t line;  // of the first pass; the next ones are side_by_side further each
     uint64_t unit;  // of the line

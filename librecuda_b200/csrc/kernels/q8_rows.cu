@@ -37,20 +37,6 @@ constexpr int kPassesUnpack = A == kWarp ? 1 : 2;
 template <int A>
 constexpr int kPassesSilu = A == kWarp ? 1 : 2;
 constexpr int kPassesGrad = 1;
-// Rows at any address give each row warps of its own from here on.  Below, lanes behind the end of a row cost more
-// than the side-by-side accesses save.  16-bit types: 333 columns of bf16 take 104 us against 82 in the gated unit,
-// 500 columns 66 against 68.  f32 with packing: 333 columns 44 us against 40 to pack, 500 columns 30 against 37;
-// without: 259 columns 41 us against 60 to unpack, 200 columns equal.
-template <typename T, bool PACKS>
-constexpr size_t kWarpColumns = sizeof(T) == 2 ? 448 : PACKS ? 400 : 224;
-// Rows that stay below: values per lane.  Loads of 32-bit values share sectors less, so fewer to a lane; stores still
-// fewer (100 columns of f32: pack 35 us with 8, 45 with 16, 40 with 4; unpack 48 with 4, 74 with 8; the 16-bit types
-// the other way round).
-template <typename T>
-constexpr int kPackForm = sizeof(T) == 4 ? kLooseShort : kLoose;
-template <typename T>
-constexpr int kStoreForm = sizeof(T) == 4 ? kLooseTiny : kLooseShort;
-
 template <typename T>
 struct Rows {  // rows of the wide type
     T *p;
@@ -72,8 +58,7 @@ struct Shape {
             const uint64_t line = kMaxThreads * Form<A>::kValues, total = (uint64_t)rows * cols, lines = (total + line - 1) / line;
             return {lines, line, line / kGroup, total, Tiling::of(lines, kMaxThreads, passes)};
         }
-        const uint64_t groups = groups_of(cols), units = groups * Form<A>::kLanes;
-        return {rows, cols, groups, 0, Tiling::of(rows, A == kWarp ? (units + 31) / 32 * 32 : units, passes)};
+        return {rows, cols, groups_of(cols), 0, Tiling::of(rows, units_of<A>(cols), passes)};
     }
 };
 
@@ -237,11 +222,11 @@ struct Fit {
         if (rows > 1 && r.stride != cols) flat = false;
     }
     void add(const Packed &p) { codes |= reinterpret_cast<uintptr_t>(p.codes); }
-    template <typename T, bool PACKS>
-    int access() const {
+    template <typename T>
+    int access(RowOp op) const {
         if (cols % 16 == 0 && wide % 32 == 0 && codes % 16 == 0) return 32;
         if (cols % 8 == 0 && wide % 16 == 0 && codes % 8 == 0) return 16;
-        return flat || cols >= kWarpColumns<T, PACKS> ? kWarp : 0;
+        return flat || warp_form_pays(op, sizeof(T) == 4, cols) ? kWarp : 0;
     }
     // one long row is addressed in lines that lie behind each other
     template <typename T>
@@ -289,7 +274,7 @@ extern "C" int lcb_pack_q8(void *codes, void *scales, const void *src, size_t sr
             Fit fit(rows, n);
             fit.add(in);
             fit.add(out);
-            return with_access<kPackForm<T>, true>(fit.template access<T, true>(), [&](auto a) {
+            return with_access<loose_form(RowOp::Pack, sizeof(T) == 4), true>(fit.template access<T>(RowOp::Pack), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesPack<a()>);
                 return with_passes<kPassesPack<a()>>(s.tiling.passes, [&](auto p) {
                     return launch_rows(pack_kernel<T, a(), p()>, s, stream, out, fit.lines(in, s));
@@ -311,7 +296,7 @@ extern "C" int lcb_unpack_q8(void *dst, size_t dst_stride, int type, const void 
             Fit fit(rows, n);
             fit.add(out);
             fit.add(in);
-            return with_access<kStoreForm<T>, true>(fit.template access<T, false>(), [&](auto a) {
+            return with_access<loose_form(RowOp::Unpack, sizeof(T) == 4), true>(fit.template access<T>(RowOp::Unpack), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesUnpack<a()>);
                 return with_passes<kPassesUnpack<a()>>(s.tiling.passes, [&](auto p) {
                     return launch_rows(unpack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), in);
@@ -338,7 +323,7 @@ extern "C" int lcb_silu_mul_pack_q8(void *h, size_t h_stride, void *gate_codes, 
             fit.add(u);
             fit.add(gp);
             fit.add(upk);
-            return with_access<kStoreForm<T>, true>(fit.template access<T, true>(), [&](auto a) {
+            return with_access<loose_form(RowOp::Unit, sizeof(T) == 4), true>(fit.template access<T>(RowOp::Unit), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesSilu<a()>);
                 return with_passes<kPassesSilu<a()>>(s.tiling.passes, [&](auto p) {
                     return launch_rows(silu_mul_pack_kernel<T, a(), p()>, s, stream, fit.lines(out, s), gp, upk, fit.lines(g, s), fit.lines(u, s));
@@ -368,7 +353,7 @@ extern "C" int lcb_silu_mul_grad_q8(void *dgate, size_t dgate_stride, void *dup,
             fit.add(d);
             fit.add(gp);
             fit.add(upk);
-            return with_access<kStoreForm<T>, true>(fit.template access<T, false>(), [&](auto a) {
+            return with_access<loose_form(RowOp::Gradient, sizeof(T) == 4), true>(fit.template access<T>(RowOp::Gradient), [&](auto a) {
                 const Shape s = Shape::of<a()>(rows, n, fit.flat, kPassesGrad);
                 return launch_rows(h != nullptr ? silu_mul_grad_kernel<T, a(), true> : silu_mul_grad_kernel<T, a(), false>, s, stream,
                                    fit.lines(dg, s), fit.lines(du, s), fit.lines(out, s), fit.lines(d, s), gp, upk);
