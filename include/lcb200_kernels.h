@@ -103,7 +103,8 @@ int lcb_axpb_f32(float *y, const float *x, float a, float b, size_t count, lcbSt
  * Outputs must not overlap each other (1 is returned where two begin at one address) nor an input, except that a
  * wide output of the two silu_mul operators may be exactly an input's rows (same address and stride).  No workspace is
  * used: calls on several streams may run at once, and a call may be captured into a CUDA graph.  A call with nothing to
- * do returns 0.
+ * do returns 0; one that would need more CTAs than a grid has (2^31 - 1; a CTA takes at least 256 values, rows padded to
+ * whole groups) returns 1.
  * ref: none (the reference has no operation that changes a format; driverapi/include/librecuda.h:37-114). */
 
 /* Writes `tokens` rows of keys and values into a paged cache, quantising them: the row of token t, head h,

@@ -8,6 +8,7 @@
 #include <initializer_list>
 
 #include "lcb200_types.h"
+#include "q8_tiling.h"
 
 namespace lcb {
 
@@ -56,12 +57,17 @@ inline bool wide_matrix_ok(const void *p, size_t stride, int type, size_t rows, 
 inline bool packed_matrix_ok(const void *codes, const void *scales, size_t rows, size_t cols) {
     return codes != nullptr && scales != nullptr && cols < SIZE_MAX - 31 && product_ok(rows, groups_of(cols), 32, 1);
 }
+// A grid has at most 2^31 - 1 CTAs.  The form with the fewest values per lane and one pass has the most.
+constexpr uint64_t kMostBlocks = 0x7fffffffu;
+inline bool grid_ok(size_t rows, size_t cols, int type) {
+    return (type == LCB_F32 ? Tiling::of(rows, units_of<kLooseTiny>(cols), 1) : Tiling::of(rows, units_of<kLooseShort>(cols), 1)).blocks() <= kMostBlocks;
+}
 
 inline bool pack_ok(const void *codes, const void *scales, const void *wide, size_t stride, int type, size_t rows, size_t cols, bool wide_is_output) {
     if (!type_ok(type)) return false;
     if (rows == 0 || cols == 0) return true;
     return codes != scales && codes != wide && scales != wide && packed_matrix_ok(codes, scales, rows, cols) &&
-           wide_matrix_ok(wide, stride, type, rows, cols, wide_is_output);
+           grid_ok(rows, cols, type) && wide_matrix_ok(wide, stride, type, rows, cols, wide_is_output);
 }
 
 inline bool silu_pack_ok(const void *h, size_t h_stride, const void *gate_codes, const void *gate_scales, const void *up_codes, const void *up_scales,
@@ -69,7 +75,7 @@ inline bool silu_pack_ok(const void *h, size_t h_stride, const void *gate_codes,
     if (!type_ok(type)) return false;
     if (rows == 0 || cols == 0) return true;
     return apart({h, gate_codes, gate_scales, up_codes, up_scales}) && packed_matrix_ok(gate_codes, gate_scales, rows, cols) &&
-           packed_matrix_ok(up_codes, up_scales, rows, cols) && wide_matrix_ok(h, h_stride, type, rows, cols, true) &&
+           packed_matrix_ok(up_codes, up_scales, rows, cols) && grid_ok(rows, cols, type) && wide_matrix_ok(h, h_stride, type, rows, cols, true) &&
            wide_matrix_ok(gate, gate_stride, type, rows, cols, false) &&
            wide_matrix_ok(up, up_stride, type, rows, cols, false);
 }
@@ -79,7 +85,7 @@ inline bool silu_grad_ok(const void *dgate, size_t dgate_stride, const void *dup
     if (!type_ok(type)) return false;
     if (rows == 0 || cols == 0) return true;
     return apart({dgate, dup, h}) && packed_matrix_ok(gate_codes, gate_scales, rows, cols) && packed_matrix_ok(up_codes, up_scales, rows, cols) &&
-           wide_matrix_ok(dgate, dgate_stride, type, rows, cols, true) && wide_matrix_ok(dup, dup_stride, type, rows, cols, true) &&
+           grid_ok(rows, cols, type) && wide_matrix_ok(dgate, dgate_stride, type, rows, cols, true) && wide_matrix_ok(dup, dup_stride, type, rows, cols, true) &&
            (h == nullptr || wide_matrix_ok(h, h_stride, type, rows, cols, true)) && wide_matrix_ok(dh, dh_stride, type, rows, cols, false);
 }
 

@@ -246,7 +246,7 @@ int in_parts(size_t rows, size_t cols, Part part) {
 template <typename... KArgs, typename... Args>
 int launch_rows(void (*kernel)(KArgs...), const Shape &s, lcbStream stream, Args... args) {
     const uint64_t blocks = s.tiling.blocks();
-    if (blocks > 0x7fffffffu) return 1;
+    if (blocks > kMostBlocks) return 1;
     return launch_kernel(kernel, (unsigned)blocks, s.tiling.threads, 0, static_cast<cudaStream_t>(stream), args..., s);
 }
 
