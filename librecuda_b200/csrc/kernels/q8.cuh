@@ -28,9 +28,13 @@ struct Lane {
     uint64_t unit;  // of the line
     bool in;        // has a unit; lanes without one still take part in a warp's votes and shuffles
     __device__ __forceinline__ Lane(const Tiling &t, uint32_t block, uint32_t passes) {
-        uint32_t chunk, place;
+        uint32_t chunk;
         const uint32_t tile = t.by_chunks.divmod(block, chunk);
+        *this = Lane(t, tile, chunk, passes);
+    }
+    __device__ __forceinline__ Lane(const Tiling &t, uint32_t tile, uint32_t chunk, uint32_t passes) {
         if (t.by_chunks.d == 1) {
+            uint32_t place;
             const uint32_t local = t.by_width.divmod(threadIdx.x, place);
             line = (uint64_t)tile * (t.side_by_side * passes) + local;
             unit = place;

@@ -46,6 +46,7 @@ struct Side {  // keys or values
     FastDiv32 per_row;               // by the units of a row, padded to whole groups
     Tiling tiling;                   // a line is a token with all its heads
     uint32_t blocks;                 // of the grid (write), or of one sequence (read); 0: no such side in this launch
+    uint64_t all_blocks() const { return dim != 0 ? tiling.blocks() : 0; }
 };
 
 struct Pool {
@@ -64,8 +65,7 @@ struct Place {
     int left;          // columns from the unit's first one on; 0: no unit
     bool leads, first; // leads its group, and so writes the scale; is the token's first unit
     template <typename T>
-    __device__ __forceinline__ Place(const Side<T> &s, uint32_t block) {
-        const Lane lane(s.tiling, block, P);
+    __device__ __forceinline__ Place(const Side<T> &s, const Lane &lane) {
         token = lane.line;
         step = s.tiling.side_by_side;
         uint32_t unit;
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
     pdl_launch_dependents();
     const bool keys = blockIdx.x < k.blocks;
     const Side<const T> s = keys ? k : v;
-    const Place<A, P> at(s, blockIdx.x - (keys ? 0 : k.blocks));
+    const Place<A, P> at(s, Lane(s.tiling, blockIdx.x - (keys ? 0 : k.blocks), P));
     const T *from = s.wide + at.token * s.token_stride + at.wide;
     uint8_t *codes = s.codes + at.code, *scales = s.scales + at.scale;
     Unit<T, A> x[P];
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
     const uint32_t in_side = block - (keys ? 0 : k.blocks);
     uint32_t chunk;
     const uint32_t run = s.tiling.by_chunks.divmod(in_side, chunk);
-    const Place<A, P> at(s, run * q.tiles * s.tiling.by_chunks.d + chunk);
+    const Place<A, P> at(s, Lane(s.tiling, run * q.tiles, chunk, P));
     const int32_t *table = q.table + b * q.table_stride;
     const uint8_t *codes = s.codes + at.code, *scales = s.scales + at.scale;
     pdl_wait();
@@ -246,7 +246,6 @@ int by_sides(const lcbCacheQ8 &c, const Wide &k, const Wide &v, size_t tokens, s
             for (Side<T> *s : {&ks, &vs}) {
                 if (s->dim == 0) continue;
                 s->tiling.passes = p;
-                s->blocks = (uint32_t)std::min<uint64_t>(s->tiling.blocks(), 0x80000000u);  // too many: refused by the launch
             }
             return with_passes<passes(a)>(p, [&](auto pp) { return launch(a, pp, ks, vs); });
         });
@@ -281,11 +280,13 @@ extern "C" int lcb_cache_write_q8(const lcbCacheQ8 *cache, const void *k, size_t
         auto passes = [](auto a) { return kPassesWrite<decltype(a)::value>; };
         return by_sides<kWriteForm<T>, T>(*cache, kw, vw, tokens, tokens, 1, passes,
                                           [&](auto a, auto p, const Side<T> &ks, const Side<T> &vs) {
-            const uint64_t blocks = (uint64_t)ks.blocks + vs.blocks;
-            if (blocks > 0x7fffffffu) return 1;
+            const uint64_t kb = ks.all_blocks(), vb = vs.all_blocks();
+            if (kb + vb > kMostBlocks) return 1;
+            Side<T> kg = ks, vg = vs;
+            kg.blocks = (uint32_t)kb, vg.blocks = (uint32_t)vb;
             const unsigned threads = std::max(ks.tiling.threads, vs.tiling.threads);
-            return launch_kernel(cache_write_kernel<std::remove_const_t<T>, a(), p()>, (unsigned)blocks, threads, 0,
-                                 static_cast<cudaStream_t>(stream), ks, vs, pool_of(*cache), slots, (uint64_t)tokens, errors);
+            return launch_kernel(cache_write_kernel<std::remove_const_t<T>, a(), p()>, (unsigned)(kb + vb), threads, 0,
+                                 static_cast<cudaStream_t>(stream), kg, vg, pool_of(*cache), slots, (uint64_t)tokens, errors);
         });
     });
 }
@@ -309,19 +310,16 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
                                         [&](auto a, auto p, const Side<T> &ks, const Side<T> &vs) {
             // Up to kRunTiles tiles to a CTA while that leaves the GPU kRunWaves grids of resident CTAs, and more of
             // them where the grid would have more than kMostWaves: max_length may be far above the lengths.
-            const uint64_t all = ((uint64_t)ks.blocks + vs.blocks) * sequences, wave = Tiling::resident_ctas();
+            const uint64_t kb = ks.all_blocks(), vb = vs.all_blocks(), all = (kb + vb) * sequences, wave = Tiling::resident_ctas();
             const uint32_t tiles = (uint32_t)std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(all / (wave * kRunWaves), 1), kRunTiles),
                                                                 std::min<uint64_t>(all / (wave * kMostWaves), 0x7fffffffu));
-            Side<T> kr = ks, vr = vs;
-            auto runs = [&](Side<T> &s) {
-                if (s.blocks == 0) return;
-                const uint64_t c = s.tiling.by_chunks.d;
-                s.blocks = (uint32_t)((s.blocks / c + tiles - 1) / tiles * c);
+            auto runs = [&](const Side<T> &s, uint64_t blocks) {  // of one sequence
+                return blocks == 0 ? 0 : (blocks / s.tiling.chunks + tiles - 1) / tiles * s.tiling.chunks;
             };
-            runs(kr);
-            runs(vr);
-            const uint64_t each = (uint64_t)kr.blocks + vr.blocks;
-            if (ks.blocks > 0x7fffffffu || vs.blocks > 0x7fffffffu || each > 0x7fffffffu || sequences > 0x7fffffffu / each) return 1;
+            const uint64_t k_runs = runs(ks, kb), v_runs = runs(vs, vb), each = k_runs + v_runs;
+            if (each > kMostBlocks || sequences > kMostBlocks / each) return 1;
+            Side<T> kr = ks, vr = vs;
+            kr.blocks = (uint32_t)k_runs, vr.blocks = (uint32_t)v_runs;
             const Sequences q{page_table, lengths, first_rows, table_stride, rows, (uint32_t)max_length, tiles, FastDiv32::of((uint32_t)each)};
             const unsigned threads = std::max(ks.tiling.threads, vs.tiling.threads);
             return launch_kernel(cache_read_kernel<T, a(), p()>, (unsigned)(each * sequences), threads, 0,

@@ -119,12 +119,29 @@ inline bool cache_rows_ok(const lcbCacheQ8 &c, const void *k, size_t kts, size_t
     };
     return side(k, kts, khs, c.k_dim) && (c.v_dim == 0 || side(v, vts, vhs, c.v_dim));
 }
+// CTAs of one line of heads in the form with the fewest values per lane that the operator takes, keys and values
+template <int A>
+uint64_t most_parts(const lcbCacheQ8 &c) {
+    uint64_t parts = 0;
+    for (size_t dim : {c.k_dim, c.v_dim})
+        if (dim != 0) parts += Tiling::of(1, c.heads * units_of<A>(dim), 1).chunks;
+    return parts;
+}
+// a write: a CTA takes at least one token of a part
+template <int A>
+uint64_t most_write_blocks(const lcbCacheQ8 &c, size_t tokens) {
+    uint64_t blocks = 0;
+    for (size_t dim : {c.k_dim, c.v_dim})
+        if (dim != 0) blocks += Tiling::of(tokens, c.heads * units_of<A>(dim), 1).blocks();
+    return blocks;
+}
 inline bool cache_write_ok(const lcbCacheQ8 *c, const void *k, size_t kts, size_t khs, const void *v, size_t vts, size_t vhs, int type,
                            const int64_t *slots, size_t tokens) {
     if (!cache_ok(c) || !type_ok(type)) return false;
     if (tokens == 0) return true;
     return apart({c->k_codes, c->k_scales, c->v_codes, c->v_scales}) && slots != nullptr && aligned(slots, 8) &&
-           cache_rows_ok(*c, k, kts, khs, v, vts, vhs, type, tokens, false);
+           cache_rows_ok(*c, k, kts, khs, v, vts, vhs, type, tokens, false) &&
+           (type == LCB_F32 ? most_write_blocks<kLooseShort>(*c, tokens) : most_write_blocks<kLoose>(*c, tokens)) <= kMostBlocks;
 }
 inline bool cache_read_ok(const lcbCacheQ8 *c, const void *k, size_t kts, size_t khs, const void *v, size_t vts, size_t vhs, int type,
                           const int32_t *table, size_t table_stride, const int32_t *lengths, const int64_t *first_rows, size_t sequences,
@@ -139,7 +156,8 @@ inline bool cache_read_ok(const lcbCacheQ8 *c, const void *k, size_t kts, size_t
     if (!aligned(table, 4) || !aligned(lengths, 4) || !aligned(first_rows, 8) || (rows >> 62)) return false;
     return product_ok(sequences, max_length, c->heads, groups_of(c->k_dim) * 32) &&
            product_ok(sequences, max_length, c->heads, groups_of(c->v_dim) * 32) &&
-           (c->v_dim == 0 || apart({k, v})) && cache_rows_ok(*c, k, kts, khs, v, vts, vhs, type, rows, true);
+           (c->v_dim == 0 || apart({k, v})) && cache_rows_ok(*c, k, kts, khs, v, vts, vhs, type, rows, true) &&
+           sequences <= (kMostBlocks - (1u << 20)) / most_parts<kLooseShort>(*c);  // the launcher shares the tokens out among 2^20 CTAs
 }
 
 }  // namespace lcb
