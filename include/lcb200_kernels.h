@@ -285,8 +285,8 @@ int lcb_device_error_peek(unsigned int *out);
  * returns.  Afterwards lcb_device_error_word reports 1 and the device is fully usable. */
 int lcb_selftest_wait_timeout(unsigned int max_tries, lcbStream stream);
 
-/* Loads the default copy / memset / fill kernels onto the current device now instead of at their first
- * launch.  ref: loadMemcpyKernelsIfNeeded, driverapi/src/memcopy.cpp:23-75, called from context creation
+/* Loads the default copy / memset / fill kernels and all forms of the 8-bit operators onto the current device now instead
+ * of at their first launch.  ref: loadMemcpyKernelsIfNeeded, driverapi/src/memcopy.cpp:23-75, called from context creation
  * (driverapi/src/librecuda.cpp:622). */
 int lcb_preload(void);
 

@@ -71,7 +71,8 @@ Tuning &tuning();
 
 int preload_copy_kernels();  // force-load the default copy / fill kernels on the current device
 int preload_fill_kernels();
-int preload_q8_kernels();
+int preload_q8_row_kernels();  // and every form of the 8-bit operators: which one a call takes goes by its addresses
+int preload_q8_cache_kernels();
 int setup_error_mirror();    // host-mapped mirror of the sticky error word for the current device
 int sm_count();            // SMs of the current device (cached per device)
 int check_launch();        // cudaGetLastError() as int

@@ -11,6 +11,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.cuh"
@@ -507,6 +508,19 @@ int with_access(int a, Fn fn) {
 template <int MOST, typename Fn>
 int with_passes(uint32_t passes, Fn fn) {
     return passes == 1 ? fn(std::integral_constant<int, 1>()) : fn(std::integral_constant<int, MOST>());
+}
+
+// Loads a kernel onto the current device, before its first launch.
+template <typename... KArgs>
+int load_kernel(void (*kernel)(KArgs...)) {
+    cudaFuncAttributes a;
+    return (int)cudaFuncGetAttributes(&a, kernel);
+}
+// the first error of a list
+inline int first_error(std::initializer_list<int> codes) {
+    for (int c : codes)
+        if (c != 0) return c;
+    return 0;
 }
 
 // ---- an index out of range in device memory -----------------------------------------------------------------------

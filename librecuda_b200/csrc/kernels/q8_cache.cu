@@ -255,11 +255,23 @@ int by_sides(const lcbCacheQ8 &c, const Wide &k, const Wide &v, size_t tokens, s
     return rc != 0 ? rc : both(va, false, true);
 }
 
+template <typename T>
+int load_cache_kernels() {
+    using C = const T;
+    constexpr int loose = kWriteForm<C>;
+    return first_error({load_kernel(cache_write_kernel<T, 32, 1>), load_kernel(cache_write_kernel<T, 32, kPassesWrite<32>>),
+                        load_kernel(cache_write_kernel<T, 16, 1>), load_kernel(cache_write_kernel<T, 16, kPassesWrite<16>>),
+                        load_kernel(cache_write_kernel<T, loose, 1>), load_kernel(cache_write_kernel<T, loose, kPassesWrite<loose>>),
+                        load_kernel(cache_read_kernel<T, 32, 1>), load_kernel(cache_read_kernel<T, 32, kPassesRead>),
+                        load_kernel(cache_read_kernel<T, 16, 1>), load_kernel(cache_read_kernel<T, 16, kPassesRead>),
+                        load_kernel(cache_read_kernel<T, kLooseShort, 1>), load_kernel(cache_read_kernel<T, kLooseShort, kPassesRead>)});
+}
+
 }  // namespace
 
-int preload_q8_kernels() {
+int preload_q8_cache_kernels() {
     ErrorSink errors;
-    return error_sink(&errors);
+    return first_error({error_sink(&errors), load_cache_kernels<float>(), load_cache_kernels<__half>(), load_cache_kernels<__nv_bfloat16>()});
 }
 }  // namespace lcb
 

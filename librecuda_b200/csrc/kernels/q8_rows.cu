@@ -257,7 +257,25 @@ Packed from(const Packed &p, size_t column) { return {p.codes + column, p.scales
 template <typename T, typename P>
 Rows<T> rows_at(P *p, size_t stride, size_t column) { return {p != nullptr ? static_cast<T *>(p) + column : nullptr, stride}; }
 
+template <typename T, int A>
+int load_pack_kernels() { return first_error({load_kernel(pack_kernel<T, A, 1>), load_kernel(pack_kernel<T, A, kPassesPack<A>>)}); }
+template <typename T, int A>
+int load_storing_kernels() {
+    return first_error({load_kernel(unpack_kernel<T, A, 1>), load_kernel(unpack_kernel<T, A, kPassesUnpack<A>>),
+                        load_kernel(silu_mul_pack_kernel<T, A, 1>), load_kernel(silu_mul_pack_kernel<T, A, kPassesSilu<A>>),
+                        load_kernel(silu_mul_grad_kernel<T, A, false>), load_kernel(silu_mul_grad_kernel<T, A, true>)});
+}
+template <typename T>
+int load_row_kernels() {
+    constexpr bool f32 = sizeof(T) == 4;
+    return first_error({load_pack_kernels<T, 32>(), load_pack_kernels<T, 16>(), load_pack_kernels<T, kWarp>(),
+                        load_pack_kernels<T, loose_form(RowOp::Pack, f32)>(), load_storing_kernels<T, 32>(), load_storing_kernels<T, 16>(),
+                        load_storing_kernels<T, kWarp>(), load_storing_kernels<T, loose_form(RowOp::Unpack, f32)>()});
+}
+
 }  // namespace
+
+int preload_q8_row_kernels() { return first_error({load_row_kernels<float>(), load_row_kernels<__half>(), load_row_kernels<__nv_bfloat16>()}); }
 }  // namespace lcb
 
 using namespace lcb;

@@ -208,7 +208,8 @@ extern "C" int lcb_tune_get(const char *name) {
 extern "C" int lcb_preload(void) {
     int rc = lcb::preload_copy_kernels();
     if (rc == 0) rc = lcb::preload_fill_kernels();
-    if (rc == 0) rc = lcb::preload_q8_kernels();
+    if (rc == 0) rc = lcb::preload_q8_row_kernels();
+    if (rc == 0) rc = lcb::preload_q8_cache_kernels();
     if (rc == 0) rc = lcb::setup_error_mirror();
     return rc;
 }
