@@ -152,19 +152,6 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
 }
 
 // ---- wide elements -------------------------------------------------------------------------------------------
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ float from_f32<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // Two values rounded to a 16-bit type, `lo` in the lower half.  FINITE: saturating at the largest finite value, what a
 // read back returns (the value of a code is at most 448 * 2^119, which only f16 cannot hold; NaN stays NaN).
 template <typename T, bool FINITE>
