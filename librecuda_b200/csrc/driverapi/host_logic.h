@@ -1,16 +1,28 @@
-// Host-side decision logic of the stream layer that needs no CUDA call to be exercised: the polling wait with
-// an optional deadline, the accumulation of event timestamps over a chain of epochs, and the record of what
-// the kernels still in flight on a lane may be writing.  Pure C++ so that tests/cpp/host_logic_test.cpp can
-// drive it on a machine without a GPU, with stubbed query functions.
+// Host-side decision logic of the stream layer that needs no CUDA call to be exercised: the words for a device
+// error, the polling wait with an optional deadline, the accumulation of event timestamps over a chain of epochs,
+// and the record of what the kernels still in flight on a lane may be writing.  Pure C++ so that programs in tests/cpp
+// can drive it on a machine without a GPU, with stubbed query functions.
 #pragma once
 
 #include <chrono>
 #include <cstddef>
 #include <cstdint>
+#include <string>
 #include <thread>
 #include <vector>
 
 namespace lcu {
+
+// ---- what the sticky device error word says ---------------------------------------------------------------
+// Bits 0 and 1: a bounded wait gave up (of a bulk copy, for another GPU's flag); bit 2: an index given in device memory
+// was out of range.
+inline std::string describe_error_word(unsigned int word) {
+    std::string s = "device error word " + std::to_string(word);
+    if (word & 3u) s += ": a kernel of this library gave up a bounded wait; its operation is incomplete";
+    if (word & 4u) s += ": a slot, page, row or length of a cache operation was out of range and was skipped";
+    if (word & ~7u) s += ": unknown bits";
+    return s;
+}
 
 // ---- polling wait ---------------------------------------------------------------------------------------
 enum class PollResult { Done, Pending, Failed };

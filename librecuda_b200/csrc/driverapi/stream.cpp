@@ -43,13 +43,14 @@ static uint64_t wait_limit_ms() {
 // A kernel of this library that gave up a bounded wait leaves its copy incomplete and raises the device's
 // sticky error word; the stream itself finishes without a CUDA error.  Checked after every host wait, so a
 // program written for the reference (which only ever looks at the status of Await) cannot take a partial
-// copy for a finished one.  The word is reported once and cleared.
+// copy for a finished one.  A cache operation that skipped an index out of range is reported the same way.  The word is
+// reported once and cleared.
 static libreCudaStatus_t check_device_error_word() {
     unsigned int w = 0;
     if (lcb_device_error_peek(&w) != 0 || w == 0) LIBRECUDA_SUCCEED();
     unsigned int cleared = 0;
     (void)lcb_device_error_word(&cleared);
-    LIBRECUDA_DEBUG("device error word " << (w | cleared) << ": a kernel of this library gave up a bounded wait; its operation is incomplete");
+    LIBRECUDA_DEBUG(describe_error_word(w | cleared));
     LIBRECUDA_FAIL(LIBRECUDA_ERROR_UNKNOWN);
 }
 
