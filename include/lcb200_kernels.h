@@ -109,8 +109,9 @@ int lcb_axpb_f32(float *y, const float *x, float a, float b, size_t count, lcbSt
 
 /* Writes `tokens` rows of keys and values into a paged cache, quantising them: the row of token t, head h,
  * k + t * k_token_stride + h * k_head_stride, goes to slot slots[t] of the cache (v likewise; v and its strides are ignored
- * in a cache of one tensor).  `slots` is DEVICE memory, 8-byte aligned.  A negative slot skips its token (a padded batch).  A slot
- * behind the last page is skipped too and raises bit 2 of the sticky error word (lcb_device_error_word).  Slots that are not
+ * in a cache of one tensor).  `slots` is DEVICE memory, 8-byte aligned.  A negative slot skips its token (a padded batch); its
+ * rows of k and v are read all the same, so they must be readable memory, whatever they hold.  A slot behind the last page is
+ * skipped too and raises bit 2 of the sticky error word (lcb_device_error_word).  Slots that are not
  * named keep their bytes.  The slots of one call must differ: a slot that is named twice holds an unspecified mix of
  * the two rows afterwards (no other slot is touched). */
 int lcb_cache_write_q8(const lcbCacheQ8 *cache, const void *k, size_t k_token_stride, size_t k_head_stride, const void *v,

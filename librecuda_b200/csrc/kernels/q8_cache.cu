@@ -94,7 +94,8 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
     int64_t slot[P];
     pdl_wait();
     // The rows of skipped tokens are loaded too: waiting for the slot first would put a second memory latency in
-    // front of every row.
+    // front of every row.  65000 tokens, a sixteenth of them skipped: 59 us, 65 with the slots first; half of them skipped
+    // 53 us, fifteen sixteenths 42.
 #pragma unroll
     for (int u = 0; u < P; ++u) {
         const uint64_t token = at.token + u * at.step;
