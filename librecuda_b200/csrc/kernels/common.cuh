@@ -14,12 +14,10 @@ constexpr unsigned int kErrMbarrierTimeout = 1u;
 constexpr unsigned int kErrFlagTimeout = 2u;
 // Bit 2: a slot, page, row or length given in device memory is out of range; it was skipped.
 constexpr unsigned int kErrIndexRange = 4u;
-// The word and the device variable that holds its host-mapped mirror (NULL before lcb_preload), as kernel arguments.
-struct ErrorSink {
-    unsigned int *word;
-    unsigned int **mirror;
-};
-int error_sink(ErrorSink *out);  // of the current device
+// The cache operators keep that bit in a word of their own source, part of the same sticky word to callers; every context
+// has its own of both.
+int index_error_mirror(unsigned int *mirror);  // host-mapped, or NULL; for the current context
+int index_error_take(unsigned int *bits);      // reads and clears
 
 // Tunables reachable through lcb_tune() (for sweeps; the defaults are the shipped configuration).
 struct Tuning {

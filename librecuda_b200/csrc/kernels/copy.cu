@@ -21,7 +21,6 @@
 //  * alltoall_kernel     one launch that moves every chunk of an all-to-all between this GPU and all its
 //                       peers (the copy fused with the exchange), by remote loads (pull) or stores (push).
 #include <cstdio>
-#include <mutex>
 
 #include "common.cuh"
 #include "lcb200_kernels.h"
@@ -1452,31 +1451,15 @@ int setup_error_mirror() {
     *h = 0;
     err = cudaHostGetDevicePointer(reinterpret_cast<void **>(&d), h, 0);
     if (err == cudaSuccess) err = cudaMemcpyToSymbol(g_error_mirror, &d, sizeof(d));
-    if (err != cudaSuccess) {
+    if (err == cudaSuccess) err = (cudaError_t)index_error_mirror(d);
+    if (err != cudaSuccess) {  // no kernel may be left with the address of memory that is freed
+        unsigned int *none = nullptr;
+        (void)cudaMemcpyToSymbol(g_error_mirror, &none, sizeof(none));
+        (void)index_error_mirror(nullptr);
         (void)cudaFreeHost(h);
         return (int)err;
     }
     g_mirror_host[dev] = h;
-    return 0;
-}
-
-// Where kernels of the other sources raise bits of the same word: the device addresses, looked up once per device.
-int error_sink(ErrorSink *out) {
-    static std::mutex guard;
-    static ErrorSink cached[64] = {};
-    int dev = -1;
-    cudaError_t err = cudaGetDevice(&dev);
-    if (err != cudaSuccess) return (int)err;
-    if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
-    const std::lock_guard<std::mutex> lock(guard);
-    if (cached[dev].word == nullptr) {
-        void *word = nullptr, *mirror = nullptr;
-        err = cudaGetSymbolAddress(&mirror, g_error_mirror);
-        if (err == cudaSuccess) err = cudaGetSymbolAddress(&word, g_error_word);
-        if (err != cudaSuccess) return (int)err;
-        cached[dev] = {static_cast<unsigned int *>(word), static_cast<unsigned int **>(mirror)};
-    }
-    *out = cached[dev];
     return 0;
 }
 }  // namespace lcb
@@ -1504,10 +1487,13 @@ extern "C" int lcb_device_error_word(unsigned int *out) {
         err = cudaMemcpyToSymbol(lcb::g_error_word, &zero, sizeof(zero));
         if (err != cudaSuccess) return (int)err;
     }
+    unsigned int index_bits = 0;
+    const int rc = lcb::index_error_take(&index_bits);
+    if (rc != 0) return rc;
     int dev = -1;
     if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 && lcb::g_mirror_host[dev] != nullptr)
         *lcb::g_mirror_host[dev] = 0;
-    *out = w;
+    *out = w | index_bits;
     return 0;
 }
 

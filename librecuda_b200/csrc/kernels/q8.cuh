@@ -510,14 +510,4 @@ inline int first_error(std::initializer_list<int> codes) {
     return 0;
 }
 
-// ---- an index out of range in device memory -----------------------------------------------------------------------
-__device__ __forceinline__ void raise_error(const ErrorSink &e, unsigned bits) {
-    atomicOr(e.word, bits);
-    unsigned int *m = *e.mirror;
-    if (m != nullptr) {
-        atomicOr_system(m, bits);
-        __threadfence_system();
-    }
-}
-
 }  // namespace lcb

@@ -23,6 +23,17 @@
 namespace lcb {
 namespace {
 
+__device__ unsigned int g_index_word = 0;              // kErrIndexRange, once an index was out of range
+__device__ unsigned int *g_index_mirror = nullptr;     // its host-mapped copy, NULL before lcb_preload
+__device__ __forceinline__ void raise_index_error() {
+    atomicOr(&g_index_word, kErrIndexRange);
+    unsigned int *m = g_index_mirror;
+    if (m != nullptr) {
+        atomicOr_system(m, kErrIndexRange);
+        __threadfence_system();
+    }
+}
+
 // Tokens in flight per lane, where there is work for that many.  Write: 4 (61 us; 2: 65; 1: 76).  Read: 2 (377 us; 4:
 // 378; 1: 422).
 template <int A>
@@ -83,7 +94,7 @@ struct Place {
 
 template <typename T, int A, int P>
 __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> k, Side<const T> v, Pool pool, const int64_t *slots,
-                                                                  uint64_t tokens, ErrorSink errors) {
+                                                                  uint64_t tokens) {
     pdl_launch_dependents();
     const bool keys = blockIdx.x < k.blocks;
     const Side<const T> s = keys ? k : v;
@@ -109,7 +120,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_write_kernel(Side<const T> 
         const unsigned b = pack_unit(x[u], c);
         if (slot[u] < 0) continue;
         if ((uint64_t)slot[u] >= pool.slots) {
-            if (at.first) raise_error(errors, kErrIndexRange);
+            if (at.first) raise_index_error();
             continue;
         }
         uint64_t page = 0, offset = (uint64_t)slot[u];  // tokens first: pages lie behind each other like their tokens
@@ -140,7 +151,7 @@ struct Sequences {
 // ends of the sequences, and a CTA that finds nothing to do costs a launch and a memory latency all the same (377 us
 // with up to 4 tiles, 404 with one, 384 with 8, which leave too few CTAs to even out the sequences).
 template <typename T, int A, int P>
-__global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side<T> v, Pool pool, Sequences q, ErrorSink errors) {
+__global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side<T> v, Pool pool, Sequences q) {
     pdl_launch_dependents();
     uint32_t block;
     const uint32_t b = q.blocks.divmod(blockIdx.x, block);
@@ -155,7 +166,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
     pdl_wait();
     const int32_t length = q.lengths[b];
     const int64_t first_row = q.first_rows[b];
-    if (block == 0 && threadIdx.x == 0 && (length < 0 || (uint32_t)length > q.max_length)) raise_error(errors, kErrIndexRange);
+    if (block == 0 && threadIdx.x == 0 && (length < 0 || (uint32_t)length > q.max_length)) raise_index_error();
     const uint32_t n = length < 0 ? 0 : min((uint32_t)length, q.max_length);
     uint32_t token = (uint32_t)at.token;
     const uint32_t tile = at.step * P, end = min((uint64_t)n, at.token + (uint64_t)tile * q.tiles);
@@ -176,7 +187,7 @@ __global__ void __launch_bounds__(kMaxThreads) cache_read_kernel(Side<T> k, Side
         for (int u = 0; u < P; ++u) {
             live[u] = at.left > 0 && token + u * at.step < n;
             if (live[u] && ((uint32_t)page[u] >= pool.pages || row + u * at.step >= q.rows)) {
-                if (at.first) raise_error(errors, kErrIndexRange);
+                if (at.first) raise_index_error();
                 live[u] = false;
             }
             if (live[u]) {
@@ -270,9 +281,16 @@ int load_cache_kernels() {
 
 }  // namespace
 
+int index_error_mirror(unsigned int *mirror) { return (int)cudaMemcpyToSymbol(g_index_mirror, &mirror, sizeof(mirror)); }
+int index_error_take(unsigned int *bits) {
+    cudaError_t err = cudaMemcpyFromSymbol(bits, g_index_word, sizeof(*bits));
+    const unsigned int zero = 0;
+    if (err == cudaSuccess && *bits != 0) err = cudaMemcpyToSymbol(g_index_word, &zero, sizeof(zero));
+    return (int)err;
+}
+
 int preload_q8_cache_kernels() {
-    ErrorSink errors;
-    return first_error({error_sink(&errors), load_cache_kernels<float>(), load_cache_kernels<__half>(), load_cache_kernels<__nv_bfloat16>()});
+    return first_error({load_cache_kernels<float>(), load_cache_kernels<__half>(), load_cache_kernels<__nv_bfloat16>()});
 }
 }  // namespace lcb
 
@@ -283,9 +301,6 @@ extern "C" int lcb_cache_write_q8(const lcbCacheQ8 *cache, const void *k, size_t
                                   lcbStream stream) {
     if (!cache_write_ok(cache, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, type, slots, tokens)) return 1;
     if (tokens == 0) return 0;
-    ErrorSink errors;
-    const int rc = error_sink(&errors);
-    if (rc != 0) return rc;
     const Wide kw{k, k_token_stride, k_head_stride, cache->k_dim, cache->k_codes, cache->k_scales};
     const Wide vw{v, v_token_stride, v_head_stride, cache->v_dim, cache->v_codes, cache->v_scales};
     return with_type(type, [&](auto *t) {
@@ -299,7 +314,7 @@ extern "C" int lcb_cache_write_q8(const lcbCacheQ8 *cache, const void *k, size_t
             kg.blocks = (uint32_t)kb, vg.blocks = (uint32_t)vb;
             const unsigned threads = std::max(ks.tiling.threads, vs.tiling.threads);
             return launch_kernel(cache_write_kernel<std::remove_const_t<T>, a(), p()>, (unsigned)(kb + vb), threads, 0,
-                                 static_cast<cudaStream_t>(stream), kg, vg, pool_of(*cache), slots, (uint64_t)tokens, errors);
+                                 static_cast<cudaStream_t>(stream), kg, vg, pool_of(*cache), slots, (uint64_t)tokens);
         });
     });
 }
@@ -311,9 +326,6 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
                        first_rows, sequences, max_length, rows))
         return 1;
     if (sequences == 0 || max_length == 0) return 0;
-    ErrorSink errors;
-    const int rc = error_sink(&errors);
-    if (rc != 0) return rc;
     const Wide kw{k, k_token_stride, k_head_stride, cache->k_dim, cache->k_codes, cache->k_scales};
     const Wide vw{v, v_token_stride, v_head_stride, cache->v_dim, cache->v_codes, cache->v_scales};
     return with_type(type, [&](auto *t) {
@@ -336,7 +348,7 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
             const Sequences q{page_table, lengths, first_rows, table_stride, rows, (uint32_t)max_length, tiles, FastDiv32::of((uint32_t)each)};
             const unsigned threads = std::max(ks.tiling.threads, vs.tiling.threads);
             return launch_kernel(cache_read_kernel<T, a(), p()>, (unsigned)(each * sequences), threads, 0,
-                                 static_cast<cudaStream_t>(stream), kr, vr, pool_of(*cache), q, errors);
+                                 static_cast<cudaStream_t>(stream), kr, vr, pool_of(*cache), q);
         });
     });
 }
