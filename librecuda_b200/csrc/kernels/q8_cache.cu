@@ -339,7 +339,7 @@ extern "C" int lcb_cache_read_q8(const lcbCacheQ8 *cache, void *k, size_t k_toke
             const uint32_t tiles = (uint32_t)std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(all / (wave * kRunWaves), 1), kRunTiles),
                                                                 std::min<uint64_t>(all / (wave * kMostWaves), 0x7fffffffu));
             auto runs = [&](const Side<T> &s, uint64_t blocks) {  // of one sequence
-                return blocks == 0 ? 0 : (blocks / s.tiling.chunks + tiles - 1) / tiles * s.tiling.chunks;
+                return blocks == 0 ? 0 : (blocks / s.tiling.by_chunks.d + tiles - 1) / tiles * s.tiling.by_chunks.d;
             };
             const uint64_t k_runs = runs(ks, kb), v_runs = runs(vs, vb), each = k_runs + v_runs;
             if (each > kMostBlocks || sequences > kMostBlocks / each) return 1;

@@ -124,7 +124,7 @@ template <int A>
 uint64_t most_parts(const lcbCacheQ8 &c) {
     uint64_t parts = 0;
     for (size_t dim : {c.k_dim, c.v_dim})
-        if (dim != 0) parts += Tiling::of(1, c.heads * units_of<A>(dim), 1).chunks;
+        if (dim != 0) parts += Tiling::of(1, c.heads * units_of<A>(dim), 1).by_chunks.d;
     return parts;
 }
 // a write: a CTA takes at least one token of a part

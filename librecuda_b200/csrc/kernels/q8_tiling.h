@@ -82,19 +82,18 @@ struct Tiling {
     uint64_t width, lines;
     FastDiv32 by_chunks, by_width;  // by_width: of lines that lie side by side, else 0 / 1
     uint32_t threads, side_by_side, passes;
-    uint64_t chunks;  // by_chunks.d where that fits its 32 bits; more make a grid that no launch takes
     // `times`: how often the launch repeats the tiling
     static Tiling of(uint64_t lines, uint64_t width, uint32_t passes, uint64_t times = 1) {
-        Tiling t{width, lines, FastDiv32::of(1), FastDiv32::of(1), 0, 1, passes, 1};
+        Tiling t{width, lines, FastDiv32::of(1), FastDiv32::of(1), 0, 1, passes};
         if (width <= kMaxThreads) {
             t.by_width = FastDiv32::of((uint32_t)width);
             t.side_by_side = (uint32_t)(kMaxThreads / width);
             if (t.side_by_side > lines) t.side_by_side = (uint32_t)lines;
             t.threads = (uint32_t)((t.side_by_side * width + 31) / 32 * 32);
         } else {
-            t.chunks = (width + kMaxThreads - 1) / kMaxThreads;
-            if (t.chunks <= 0xffffffffu) t.by_chunks = FastDiv32::of((uint32_t)t.chunks);
-            t.threads = (uint32_t)(((width + t.chunks - 1) / t.chunks + 31) / 32 * 32);
+            const uint64_t chunks = (width + kMaxThreads - 1) / kMaxThreads;
+            t.by_chunks = FastDiv32::of(chunks < 0xffffffffu ? (uint32_t)chunks : 0xffffffffu);  // so many: no launch takes the grid
+            t.threads = (uint32_t)(((width + chunks - 1) / chunks + 31) / 32 * 32);
         }
         if (passes > 1 && t.blocks() * times < resident_ctas() / 2) t.passes = 1;
         return t;
@@ -102,7 +101,7 @@ struct Tiling {
     static uint64_t resident_ctas() { return (uint64_t)sm_count() * (2048 / kMaxThreads); }
     uint64_t blocks() const {
         const uint64_t tile = (uint64_t)side_by_side * passes;
-        return (lines + tile - 1) / tile * chunks;
+        return (lines + tile - 1) / tile * by_chunks.d;
     }
 };
 
