@@ -10,8 +10,9 @@
 // beside their slots.
 //
 // Measured on a B200 (bf16, 8 heads of 128; share of 6548 GB/s): write of 65000 tokens, a sixteenth of them padding,
-// 61 us, 95 % (65 us and 89 % heads first: 128-byte pieces); read of 48 sequences of 1 to 16384 tokens 377 us, 99 %;
-// in f32 100 %.  Heads of 65: 83 us and 36 %, 517 us and 37 %, rows at any address that are too short for a warp.
+// 60 us, 96 % (64 us and 90 % heads first: 128-byte pieces); read of 48 sequences of 1 to 16384 tokens 377 us, 99 %;
+// in f32 99 %.  A cache of one tensor, 576 wide: 20.7 us and 84 %, 117 us and 90 %.  Heads of 65: 84 us and 35 %, 515 us and
+// 37 %, rows at any address in words lane by lane.
 // One token: write 1.05 us in a graph. One lane per value instead of 16: 997 and 9805 us.  Rows loaded only once
 // their slots are known: 65 us against 61.
 #include <algorithm>

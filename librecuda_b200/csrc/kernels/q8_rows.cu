@@ -15,10 +15,11 @@
 // Measured on a B200 (bf16 unless said; share of 6548 GB/s, what a copy of the same bytes by torch reaches): pack
 // 16384 x 8192 59 us, 105 %; unpack 61 us, 102 %; unpack 16400 x 5120 to f32 63.6 us, 101 %; gated unit 8192 x 10240
 // 101 us, 102 %; its gradient with h again 125.5 us, 103 %, without 101 us.  Rows of 16-byte alignment: pack 16384 x
-// 8200 69 us, 91 %.  Rows at any address: pack 16384 x 8191 102 us, unpack 86 us, gated unit 8192 x 10241 195 us,
-// gradient 172 us: 53-72 %, bound by issue slots and L1 accesses; f32 with 1001 columns: pack 32, unpack 29 of 23
-// us.  Smallest calls: 1.1-1.6 us in a graph. One lane per value instead of 16: pack 542 us, unpack to f32 339, gated
-// unit 503, gradient 405.
+// 8200 67 us, 93 %.  Rows at any address: pack 16384 x 8191 101-104 us, unpack 88 us, gated unit 8192 x 10241 194 us,
+// gradient 175 us: 53-70 %, held by two to three times the instructions and, but for unpack, by a third of the warps that an
+// SM holds; f32 with 1001 columns: pack 32, unpack 29 of 23 us.  Small calls in a graph: unpack of a row 1.1 us, pack 129 x
+// 1001 and the gated unit 7 x 1416 1.7, gradient 33 x 2731 3.0.  One lane per value instead of 16: pack 542 us, unpack to
+// f32 339, gated unit 503, gradient 405.
 #include "lcb200_kernels.h"
 #include "q8.cuh"
 #include "q8_check.h"
@@ -27,9 +28,10 @@ namespace lcb {
 namespace {
 
 // Units in flight per lane, where there is work for that many.  Pack: 4 (59.1 us; 3 and 2 within 1 %, 1: 64).
-// Unpack: 2 (60.9 us; 1: 69), in the warp form 1 (84.7 us at 16384 x 8191; 2: 86.9).  Gated unit: 2 of each input (101
-// us; 1: 106), in the warp form 1 (201 us; 2: 236, whose loads no longer fit L1).  Gradient: 1, which already has three
-// inputs in flight and three outputs to hold; 2 take 86 registers and 169 us against 125.
+// Unpack: 2 (60.9 us; 1: 69), in the warp form 1 (88 us at 16384 x 8191; 2 within 1 %).  Gated unit: 2 of each input
+// (101 us; 1: 106), in the warp form 1, its registers held to 6 CTAs per SM (194 us at 8192 x 10241, 201 without that limit;
+// 2: 226 and 236, whose loads no longer fit L1).  Gradient: 1, which already has three inputs in flight and three outputs to
+// hold; 2 take 86 registers and 169 us against 125.
 template <int A>
 constexpr int kPassesPack = A >= 16 ? 4 : 2;
 template <int A>
